@@ -1,0 +1,236 @@
+// Dense products beside the packed experts, grouped by expert: entry points, the kernel that takes every shape, and the weighted
+// sum over a token's experts.
+//   y[i] = x[row(i)] . W[e(i)]^T                                                             (bm_grouped_linear)
+//   y[t] = residual[t] + sum_s w[t, s] * Wd[e] . (silu(Wg[e] . x[t]) * (Wu[e] . x[t]))       (bm_dense_experts_forward)
+// The second is what a block runs for its un-quantised ("super") experts, which the reference runs one module at a time on the rows
+// that torch.nonzero finds (bitsmoe/models/base_block.py:291-313): routing build, gate and up products with silu * mul, down products,
+// weighted sum, on one stream and without a host round trip.
+#include "grouped.cuh"
+
+namespace bm {
+
+constexpr int GG_ROWS = 16, GG_COLS = 64, GG_K = 32, GG_THREADS = 256;
+
+template <int D>
+__device__ __forceinline__ float load16(const void* p, int64_t i) {
+  return D == BM_F16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Any shape and alignment: a CTA takes 16 rows of a group and 64 output columns, element loads, fp32 FMA.
+template <int D, bool GLU>
+__global__ void __launch_bounds__(GG_THREADS) grouped_any_kernel(const GroupedArgs a) {
+  __shared__ float xs[GG_K][GG_ROWS + 1], ws[GLU ? 2 : 1][GG_K][GG_COLS + 1];
+  __shared__ int found[3];
+  __shared__ int src[GG_ROWS];
+  const int lane = threadIdx.x & 31, n0 = blockIdx.x * GG_COLS;
+  grid_launch_dependents();
+  grid_wait();
+  for (int64_t tile = blockIdx.y;; tile += gridDim.y) {
+    // the group of row tile `tile`: 32 groups at a time
+    if (threadIdx.x < 32) {
+      int64_t before = 0;
+      if (lane == 0) found[0] = -1;
+      for (int e0 = 0; e0 < a.E; e0 += 32) {
+        const int e = e0 + lane;
+        const int2 r = e < a.E ? group_rows(a.offsets, e, a.rows) : make_int2(0, 0);
+        const int n = (r.y - r.x + GG_ROWS - 1) / GG_ROWS;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const int64_t first = before + incl - n;
+        if (tile >= first && tile < first + n) {
+          found[0] = e;
+          found[1] = r.x + static_cast<int>(tile - first) * GG_ROWS;
+          found[2] = r.y;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+        if (before > tile) break;
+      }
+    }
+    __syncthreads();
+    const int e = found[0], row0 = found[1], rows = min(GG_ROWS, found[2] - row0);
+    if (e < 0) return;
+    if (threadIdx.x < GG_ROWS) {
+      int r = -1;
+      if (threadIdx.x < rows) r = a.index ? __ldg(a.index + row0 + threadIdx.x) : row0 + threadIdx.x;
+      src[threadIdx.x] = r >= 0 && r < a.x_rows ? r : -1;
+    }
+    __syncthreads();
+    const int col = threadIdx.x & 63, rg = threadIdx.x >> 6;      // four rows of one column
+    const int64_t w0 = static_cast<int64_t>(e) * (GLU ? 2 : 1) * a.N;
+    float acc[GLU ? 2 : 1][4] = {};
+    for (int k0 = 0; k0 < a.K; k0 += GG_K) {
+      for (int i = threadIdx.x; i < GG_ROWS * GG_K; i += GG_THREADS) {
+        const int r = i / GG_K, k = i % GG_K;
+        xs[k][r] = src[r] >= 0 && k0 + k < a.K ? load16<D>(a.x, static_cast<int64_t>(src[r]) * a.K + k0 + k) : 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < (GLU ? 2 : 1); ++h)
+        for (int i = threadIdx.x; i < GG_COLS * GG_K; i += GG_THREADS) {
+          const int c = i / GG_K, k = i % GG_K;
+          ws[h][k][c] = n0 + c < a.N && k0 + k < a.K ? load16<D>(a.w, (w0 + static_cast<int64_t>(h) * a.N + n0 + c) * a.K + k0 + k) : 0.f;
+        }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < GG_K; ++k)
+#pragma unroll
+        for (int h = 0; h < (GLU ? 2 : 1); ++h) {
+          const float w = ws[h][k][col];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[h][j] = fmaf(xs[k][4 * rg + j], w, acc[h][j]);
+        }
+      __syncthreads();
+    }
+    if (n0 + col < a.N)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * rg + j < rows)
+          store_act(a.y, a.y_dtype, static_cast<int64_t>(row0 + 4 * rg + j) * a.N + n0 + col, GLU ? silu_mul(acc[0][j], acc[GLU ? 1 : 0][j]) : acc[0][j]);
+    __syncthreads();
+  }
+}
+
+int launch_grouped(const GroupedArgs& a, cudaStream_t st) {
+  if (a.rows == 0 || a.E == 0) return BM_OK;
+  const int64_t tiles = a.rows / GG_ROWS + static_cast<int64_t>(a.E < a.rows ? a.E : a.rows) + 1;
+  const dim3 grid((a.N + GG_COLS - 1) / GG_COLS, static_cast<unsigned>(tiles < 65535 ? tiles : 65535));
+  auto* kernel = a.dtype == BM_F16 ? (a.glu ? grouped_any_kernel<BM_F16, true> : grouped_any_kernel<BM_F16, false>)
+                                   : (a.glu ? grouped_any_kernel<BM_BF16, true> : grouped_any_kernel<BM_BF16, false>);
+  BM_CUDA(launch_after(a.after, 1, kernel, grid, GG_THREADS, 0, st, a));
+  BM_LAUNCH_CHECK("grouped_any_kernel");
+  return BM_OK;
+}
+
+// y[t] = residual[t] + sum over the slots s of w[t, s] * d[position of (t, s)], in the order of the slots.  A token's place in its
+// expert's list is found by bisection: the routing build keeps the lists in ascending (token, slot) order.
+constexpr int EC_THREADS = 128, EC_MAX_K = 32;
+struct CombineArgs {
+  const float* d;              // [T * k, H] in expert order
+  const int32_t *topk_idx, *map, *token_indices, *offsets;
+  const float* topk_w;
+  const void* residual;
+  void* y;
+  int T, k, H, E, num_routed, dtype;
+};
+__global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const CombineArgs a) {
+  __shared__ int local[EC_MAX_K], at[EC_MAX_K];
+  __shared__ float weight[EC_MAX_K];
+  const int t = blockIdx.x, s = threadIdx.x;
+  grid_launch_dependents();
+  grid_wait();
+  if (s < a.k) {
+    const int id = a.topk_idx[static_cast<int64_t>(t) * a.k + s];
+    int e = id >= 0 && id < a.num_routed ? (a.map ? a.map[id] : id) : -1;
+    if (e >= a.E) e = -1;
+    local[s] = e;
+    weight[s] = a.topk_w[static_cast<int64_t>(t) * a.k + s];
+  }
+  __syncthreads();
+  if (s < a.k) {
+    const int e = local[s];
+    int lo = 0;
+    if (e >= 0) {
+      int hi = a.offsets[e + 1];
+      lo = a.offsets[e];
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.token_indices[mid] < t) lo = mid + 1;
+        else hi = mid;
+      }
+      for (int p = 0; p < s; ++p) lo += local[p] == e;      // an expert may be named twice
+    }
+    at[s] = lo;
+  }
+  __syncthreads();
+  for (int h = threadIdx.x; h < a.H; h += EC_THREADS) {
+    const int64_t o = static_cast<int64_t>(t) * a.H + h;
+    float v = a.residual ? load_act(a.residual, a.dtype, o) : 0.f;
+    for (int j = 0; j < a.k; ++j)
+      if (local[j] >= 0) v = fmaf(weight[j], a.d[static_cast<int64_t>(at[j]) * a.H + h], v);
+    store_act(a.y, a.dtype, o, v);
+  }
+}
+
+struct DenseExpertsWs {
+  size_t tok, rw, off, route, z, d, total;
+  DenseExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    const size_t A = static_cast<size_t>(T * k);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += align_up(bytes, 256);
+      return here;
+    };
+    tok = take(A * 4);
+    rw = take(A * 4);
+    off = take(static_cast<size_t>(E + 1) * 4);
+    route = take(bm_route_build_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(k), static_cast<int32_t>(E)));
+    z = take(A * I * 2);
+    d = take(A * H * 4);
+    total = at;
+  }
+};
+
+}  // namespace bm
+
+using namespace bm;
+
+extern "C" int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_rows, int32_t K, int32_t N, int32_t E,
+                                 const int32_t* expert_offsets, const int32_t* token_indices, int32_t rows, void* y, void* stream) {
+  bm::NvtxRange nvtx_range("bm_grouped_linear");
+  BM_REQUIRE(x_rows >= 0 && rows >= 0 && K > 0 && N > 0 && E >= 0, BM_ERR_INVALID_ARG, "grouped_linear: bad sizes");
+  BM_REQUIRE(dtype == BM_F16 || dtype == BM_BF16, BM_ERR_INVALID_ARG, "grouped_linear: x and the weights must be fp16 or bf16");
+  if (rows == 0 || E == 0) return BM_OK;
+  BM_REQUIRE((x || x_rows == 0) && w && expert_offsets && y, BM_ERR_INVALID_ARG, "grouped_linear: null pointer");
+  BM_REQUIRE(token_indices || rows <= x_rows, BM_ERR_INVALID_ARG, "grouped_linear: %d rows without indices, x has %d", rows, x_rows);
+  GroupedArgs a{};
+  a.x = x; a.w = w; a.offsets = expert_offsets; a.index = token_indices; a.y = y;
+  a.x_rows = x_rows; a.rows = rows; a.K = K; a.N = N; a.E = E; a.dtype = a.y_dtype = dtype;
+  return launch_grouped(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t bm_dense_experts_workspace_bytes(int32_t T, int32_t k, int32_t num_local, int32_t hidden, int32_t intermediate) {
+  if (T <= 0 || k <= 0 || num_local <= 0 || hidden <= 0 || intermediate <= 0) return 0;
+  return DenseExpertsWs(T, k, num_local, hidden, intermediate).total;
+}
+
+extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t* topk_idx, const float* topk_w, const int32_t* global_to_local,
+                                        int32_t num_routed, int32_t T, int32_t k, int32_t num_local, const void* w_gate_up, const void* w_down,
+                                        int32_t hidden, int32_t intermediate, const void* residual, void* y, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  bm::NvtxRange nvtx_range("bm_dense_experts_forward");
+  BM_REQUIRE(T >= 0 && k > 0 && num_local > 0 && num_routed > 0 && hidden > 0 && intermediate > 0, BM_ERR_INVALID_ARG, "dense_experts: bad sizes");
+  BM_REQUIRE(dtype == BM_F16 || dtype == BM_BF16, BM_ERR_INVALID_ARG, "dense_experts: x and the weights must be fp16 or bf16");
+  BM_REQUIRE(k <= EC_MAX_K, BM_ERR_UNSUPPORTED, "dense_experts: top_k=%d exceeds %d", k, EC_MAX_K);
+  BM_REQUIRE(static_cast<int64_t>(T) * k < (1ll << 30), BM_ERR_UNSUPPORTED, "dense_experts: too many assignments");
+  if (T == 0) return BM_OK;
+  BM_REQUIRE(x && topk_idx && topk_w && w_gate_up && w_down && y, BM_ERR_INVALID_ARG, "dense_experts: null pointer");
+  const DenseExpertsWs at(T, k, num_local, hidden, intermediate);
+  BM_REQUIRE(workspace && workspace_bytes >= at.total && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, BM_ERR_WORKSPACE,
+             "dense_experts: workspace must be 256-byte aligned and hold %zu bytes (%zu given)", at.total, workspace_bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  int32_t *tok = reinterpret_cast<int32_t*>(ws + at.tok), *off = reinterpret_cast<int32_t*>(ws + at.off);
+  const int A = T * k;
+  int rc = bm_route_build(topk_idx, topk_w, global_to_local, num_routed, T, k, num_local, 128, tok, off, reinterpret_cast<float*>(ws + at.rw), nullptr,
+                          nullptr, ws + at.route, at.z - at.route, stream);
+  if (rc) return rc;
+  GroupedArgs g{};
+  g.x = x; g.w = w_gate_up; g.offsets = off; g.index = tok; g.y = ws + at.z;
+  g.x_rows = T; g.rows = A; g.K = hidden; g.N = intermediate; g.E = num_local; g.dtype = g.y_dtype = dtype; g.glu = 1;
+  g.after = AFTER_READS;
+  if ((rc = launch_grouped(g, st))) return rc;
+  g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
+  g.x_rows = A; g.K = intermediate; g.N = hidden; g.glu = 0;
+  if ((rc = launch_grouped(g, st))) return rc;
+  CombineArgs c{};
+  c.d = reinterpret_cast<const float*>(ws + at.d);
+  c.topk_idx = topk_idx; c.map = global_to_local; c.token_indices = tok; c.offsets = off; c.topk_w = topk_w;
+  c.residual = residual; c.y = y; c.T = T; c.k = k; c.H = hidden; c.E = num_local; c.num_routed = num_routed; c.dtype = dtype;
+  BM_CUDA(launch_after(AFTER_READS, 1, experts_combine_kernel, dim3(T), EC_THREADS, 0, st, c));
+  BM_LAUNCH_CHECK("experts_combine_kernel");
+  return BM_OK;
+}

@@ -1,0 +1,34 @@
+// Products of rows grouped by expert (grouped.cu, grouped_tc.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace bm {
+
+// y[i][n] = sum_k x[row(i)][k] * w[e][n][k] for offsets[e] <= i < offsets[e + 1], row(i) = index[i] (i itself when null).
+// glu: w holds 2 N rows per expert, gate rows before up rows, and y[i][n] = silu(row n) * row (N + n).
+// offsets null: one group of all `rows` rows.
+struct GroupedArgs {
+  const void* x;               // [x_rows, K]
+  const void* w;               // [E, N or 2 N, K], of x's type
+  const int32_t* offsets;      // [E + 1], device
+  const int32_t* index;        // [rows], device; entries outside [0, x_rows) stand for rows of zeros
+  void* y;                     // [rows, N]
+  int x_rows, rows, K, N, E;
+  int dtype, y_dtype;          // of x and w: BM_F16 or BM_BF16; of y: the same or BM_F32
+  int glu;
+  LaunchAfter after;
+};
+
+// The rows of group e, whatever the caller's table holds: inside [0, rows), ends not before they start.
+__device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int rows) {
+  if (!offsets) return make_int2(0, rows);
+  const int a = min(max(__ldg(offsets + e), 0), rows);
+  return make_int2(a, min(max(__ldg(offsets + e + 1), a), rows));
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+int launch_grouped(const GroupedArgs& a, cudaStream_t st);
+
+}  // namespace bm

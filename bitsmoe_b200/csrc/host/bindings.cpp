@@ -6,6 +6,7 @@
 // The semantics are those of bitsmoe_b200/layer.py, which calls these functions.
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -297,6 +298,85 @@ PyObject* dense_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- dense products grouped by expert
+void refuse_grad(const char* what, std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) fail(PyExc_RuntimeError, std::string(what) + " has no backward pass: call it under torch.no_grad(), or on detached tensors");
+}
+int half_code(const at::Tensor& t, const char* msg) {
+  require(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, msg);
+  return dtype_code(t.scalar_type());
+}
+void require_int32_range(int64_t v, const char* msg) { require(v <= 0x7fffffff, msg); }
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+  return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, like.options().dtype(at::kByte));
+}
+
+// (x [T, K], weight [E, N, K], expert_offsets int32 [E + 1], token_indices int32 [rows] | None, out [rows, N] | None) -> y
+PyObject* grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 5);
+    const at::Tensor x = contiguous(tensor(a[0])), w = contiguous(tensor(a[1])), off = tensor(a[2]), tok = opt_tensor(a[3]), out = opt_tensor(a[4]);
+    require_cuda(x, "grouped_linear");
+    refuse_grad("grouped_linear", {&x, &w, &out});
+    const int dtype = half_code(x, "grouped_linear: x must be float16 or bfloat16");
+    require(w.device() == x.device() && w.scalar_type() == x.scalar_type(), "grouped_linear: the weights must have x's type and device");
+    require(x.dim() == 2 && w.dim() == 3 && w.size(2) == x.size(1) && w.size(1) > 0 && w.size(2) > 0, "grouped_linear: x must be [T, K] and weight [E, N, K]");
+    require(off.device() == x.device() && off.scalar_type() == at::kInt && off.is_contiguous() && off.dim() == 1 && off.numel() == w.size(0) + 1,
+            "grouped_linear: expert_offsets must be contiguous int32 [experts + 1] on x's device");
+    require(!tok.defined() || (tok.device() == x.device() && tok.scalar_type() == at::kInt && tok.is_contiguous() && tok.dim() == 1),
+            "grouped_linear: token_indices must be a contiguous int32 vector on x's device");
+    const int64_t rows = tok.defined() ? tok.numel() : x.size(0);
+    for (int64_t v : {x.size(0), x.size(1), w.size(0), w.size(1), rows}) require_int32_range(v, "grouped_linear: a size exceeds 32 bits");
+    require(!out.defined() || (out.device() == x.device() && out.scalar_type() == x.scalar_type() && out.is_contiguous() && out.dim() == 2 &&
+                               out.size(0) == rows && out.size(1) == w.size(1)),
+            "grouped_linear: out must be contiguous [rows, N] of x's type and device");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor y = out.defined() ? out : at::empty({rows, w.size(1)}, x.options());
+    check(bm_grouped_linear(x.data_ptr(), dtype, w.data_ptr(), static_cast<int32_t>(x.size(0)), static_cast<int32_t>(x.size(1)),
+                            static_cast<int32_t>(w.size(1)), static_cast<int32_t>(w.size(0)), static_cast<const int32_t*>(off.data_ptr()),
+                            static_cast<const int32_t*>(ptr(tok)), static_cast<int32_t>(rows), y.data_ptr(), stream_of(x.device())));
+    return THPVariable_Wrap(y);
+  });
+}
+
+// (x [T, H], topk_idx [T, k], topk_w [T, k], w_gate_up [E, 2 I, H], w_down [E, H, I], global_to_local | None, residual | None) -> y
+PyObject* dense_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 7);
+    const at::Tensor x = contiguous(tensor(a[0])), gu = contiguous(tensor(a[3])), dn = contiguous(tensor(a[4])), g2l = opt_tensor(a[5]);
+    at::Tensor idx = tensor(a[1]), w = tensor(a[2]), residual = opt_tensor(a[6]);
+    require_cuda(x, "dense_experts");
+    refuse_grad("dense_experts", {&x, &w, &gu, &dn, &residual});
+    const int dtype = half_code(x, "dense_experts: x must be float16 or bfloat16");
+    for (const at::Tensor* t : {&gu, &dn})
+      require(t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->dim() == 3, "dense_experts: the weights must be three-dimensional, of x's type and device");
+    require(x.dim() == 2 && gu.size(0) == dn.size(0) && gu.size(2) == x.size(1) && dn.size(1) == x.size(1) && gu.size(1) == 2 * dn.size(2) && gu.size(0) > 0 &&
+                dn.size(2) > 0 && x.size(1) > 0,
+            "dense_experts: x must be [T, H], w_gate_up [E, 2 I, H] and w_down [E, H, I]");
+    require(idx.dim() == 2 && w.dim() == 2 && idx.sizes() == w.sizes() && idx.size(0) == x.size(0) && idx.size(1) > 0 && idx.device() == x.device() &&
+                w.device() == x.device() && (idx.scalar_type() == at::kInt || idx.scalar_type() == at::kLong) && w.is_floating_point(),
+            "dense_experts: topk_idx (int32 or int64) and topk_w must be [T, k] on x's device");
+    const int64_t T = x.size(0), k = idx.size(1), E = gu.size(0), H = x.size(1), I = dn.size(2), routed = g2l.defined() ? g2l.numel() : E;
+    for (int64_t v : {T, k, E, H, 2 * I, routed}) require_int32_range(v, "dense_experts: a size exceeds 32 bits");
+    require_map(g2l, routed, x.device());
+    require_residual(residual, x);
+    const c10::cuda::CUDAGuard guard(x.device());
+    idx = contiguous(idx.scalar_type() == at::kInt ? idx : idx.clamp(-1, 0x7fffffff).to(at::kInt));
+    w = contiguous(w.scalar_type() == at::kFloat ? w : w.to(at::kFloat));
+    if (residual.defined()) residual = contiguous(residual.scalar_type() == x.scalar_type() ? residual : residual.to(x.scalar_type()));
+    const at::Tensor y = at::empty_like(x);
+    const int32_t T32 = static_cast<int32_t>(T), k32 = static_cast<int32_t>(k), E32 = static_cast<int32_t>(E), H32 = static_cast<int32_t>(H), I32 = static_cast<int32_t>(I);
+    const size_t need = bm_dense_experts_workspace_bytes(T32, k32, E32, H32, I32);
+    const at::Tensor ws = scratch(need, x);
+    check(bm_dense_experts_forward(x.data_ptr(), dtype, static_cast<const int32_t*>(idx.data_ptr()), static_cast<const float*>(w.data_ptr()),
+                                   static_cast<const int32_t*>(ptr(g2l)), static_cast<int32_t>(routed), T32, k32, E32, gu.data_ptr(), dn.data_ptr(), H32, I32,
+                                   ptr(residual), y.data_ptr(), ws.data_ptr(), ws.nbytes(), stream_of(x.device())));
+    return THPVariable_Wrap(y);
+  });
+}
+
 at::Tensor run_experts(HostLayer* L, const at::Tensor& hg, const at::Tensor& hu, const at::Tensor& tok, const at::Tensor& off,
                        const at::Tensor& rw, int64_t rank_out, int32_t path) {
   // h_up may have fewer rows than h_gate: only the rows that token_indices names are read
@@ -522,7 +602,7 @@ PyObject* pack_matrix(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(layer_new), FAST(layer_close), FAST(layer_drop_workspaces), FAST(layer_workspace), FAST(layer_forward),
-                         FAST(block_forward), FAST(dense_mlp), FAST(experts_forward), FAST(op_forward), FAST(op_register), FAST(pack_matrix),
+                         FAST(block_forward), FAST(dense_mlp), FAST(grouped_linear), FAST(dense_experts), FAST(experts_forward), FAST(op_forward), FAST(op_register), FAST(pack_matrix),
                          {"op_clear", op_clear, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bm_host", "Native host path of bitsmoe_b200.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

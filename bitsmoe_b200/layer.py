@@ -293,3 +293,26 @@ def dense_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if not x.is_cuda:
         raise RuntimeError("dense_mlp requires CUDA tensors; there is no CPU path")
     return capi.host().dense_mlp(x, w_gate, w_up, w_down, None if token_gate_weight is None else token_gate_weight.reshape(-1), residual)
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, expert_offsets: torch.Tensor, token_indices: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows grouped by expert times their expert's matrix: y[i] = x[row(i)] @ weight[e].T for expert_offsets[e] <= i <
+    expert_offsets[e + 1], with row(i) = token_indices[i], or i without indices.  x [T, K] and weight [E, N, K] fp16 or bf16 (one
+    type), ``expert_offsets`` int32 [E + 1] and ``token_indices`` int32 [rows] as ``route_build`` gives them -> [rows, N].  No host
+    sync; forward only.  Rows that no expert owns (behind expert_offsets[-1]) stay as they were in ``out`` and are unspecified
+    without it; an index outside x stands for a row of zeros."""
+    if not x.is_cuda:
+        raise RuntimeError("grouped_linear requires CUDA tensors; there is no CPU path")
+    return capi.host().grouped_linear(x, weight, expert_offsets, token_indices, out)
+
+
+def dense_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
+                  global_to_local: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Un-quantised SwiGLU experts for a given selection: y[t] = residual[t] + sum over slots of topk_w[t, s] * expert(x[t]).  x [T, H]
+    fp16 or bf16, w_gate_up [E, 2I, H] (gate rows before up rows) and w_down [E, H, I] of x's type, topk_idx and topk_w [T, k] with
+    k <= 32; ``global_to_local`` int32 maps routed ids to the E experts held here, anything else to -1 (those slots add nothing).
+    No host sync; the sum runs in the order of the slots, in fp32; forward only."""
+    if not x.is_cuda:
+        raise RuntimeError("dense_experts requires CUDA tensors; there is no CPU path")
+    return capi.host().dense_experts(x, topk_idx, topk_w, w_gate_up, w_down, global_to_local, residual)

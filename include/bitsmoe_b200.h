@@ -254,6 +254,25 @@ BM_API int bm_dense_mlp_forward(const void* x, int x_dtype, const uint16_t* w_ga
                                 const uint16_t* token_gate_w, int32_t T, int32_t hidden, int32_t intermediate,
                                 const void* residual, void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- products grouped by expert ------------------------------------------
+ * Un-quantised experts beside the packed ones, fp16 or bf16 (`dtype`: of activations, weights and outputs; sums are fp32).
+ * y[i] = x[row(i)] . w[e]^T for expert_offsets[e] <= i < expert_offsets[e + 1]: w [E, N, K], y [rows, N], row(i) = token_indices[i]
+ * (int32 [rows]; an entry outside [0, x_rows) stands for a row of zeros), or i where token_indices is NULL (then rows <= x_rows).
+ * expert_offsets int32 [E + 1] on the device, ascending; entries are limited to [0, rows].  Rows of y that no expert owns, such as
+ * those behind expert_offsets[E], are left as they were. */
+BM_API int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_rows, int32_t K, int32_t N, int32_t E,
+                             const int32_t* expert_offsets, const int32_t* token_indices, int32_t rows, void* y, void* stream);
+/* Dense SwiGLU experts of a MoE block for a given selection (_run_super_experts of bitsmoe/models/base_block.py:291-307, without its
+ * host round trips):  y[t] = residual[t] + sum over slots s of topk_w[t, s] * w_down[e] . (silu(gate_e . x[t]) * (up_e . x[t])),
+ * e = global_to_local[topk_idx[t, s]] (the id itself when the map is NULL, and then num_routed must equal num_local); slots whose id
+ * is not held here add nothing.  w_gate_up [num_local, 2 * intermediate, hidden], gate rows before up rows; w_down [num_local, hidden,
+ * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits. */
+BM_API size_t bm_dense_experts_workspace_bytes(int32_t T, int32_t k, int32_t num_local, int32_t hidden, int32_t intermediate);
+BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* topk_idx, const float* topk_w, const int32_t* global_to_local,
+                                    int32_t num_routed, int32_t T, int32_t k, int32_t num_local, const void* w_gate_up,
+                                    const void* w_down, int32_t hidden, int32_t intermediate, const void* residual, void* y,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- whole block -------------------------------------------------------
  * The dense parts of a block beside its packed experts, in the model's own type (w_dtype: BM_F16, or BM_BF16, which is
  * rounded to fp16 on the way to the tensor cores); pointers that are NULL are left out.  `gate_w` [num_routed, hidden] is
