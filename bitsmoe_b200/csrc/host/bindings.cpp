@@ -377,6 +377,75 @@ PyObject* dense_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- products with 4-bit weights
+// A packed matrix [n, k]: what bm_linear4 says of payload and scale.
+void require_matrix4(const at::Tensor& p, const at::Tensor& s, int64_t n, int64_t k, int64_t group, const at::Tensor& x, const char* msg) {
+  require(p.device() == x.device() && s.device() == x.device() && p.scalar_type() == at::kUInt32 && s.scalar_type() == at::kHalf && p.is_contiguous() &&
+              s.is_contiguous() && p.dim() == 2 && s.dim() == 2 && p.size(0) == n && s.size(0) == n && p.size(1) == (k + 31) / 32 * 4 &&
+              s.size(1) == (k + group - 1) / group,
+          msg);
+}
+int32_t group_size(PyObject* o) {
+  const long g = integer(o);
+  require(g == 32 || g == 64 || g == 128, "group_size must be 32, 64 or 128");
+  return static_cast<int32_t>(g);
+}
+
+// (x [T, K], payload, scale, group size, residual | None) -> y [T, N]
+PyObject* linear4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 5);
+    const at::Tensor x = contiguous(tensor(a[0])), &p = tensor(a[1]), &s = tensor(a[2]);
+    const int32_t group = group_size(a[3]);
+    at::Tensor residual = opt_tensor(a[4]);
+    require_cuda(x, "linear4");
+    refuse_grad("linear4", {&x, &s, &residual});
+    const int dtype = half_code(x, "linear4: x must be float16 or bfloat16");
+    require(x.dim() == 2 && x.size(1) > 0 && p.dim() == 2 && p.size(0) > 0, "linear4: x must be [T, K] and the matrix have rows");
+    const int64_t T = x.size(0), K = x.size(1), N = p.size(0);
+    for (int64_t v : {T, K, N}) require_int32_range(v, "linear4: a size exceeds 32 bits");
+    require_matrix4(p, s, N, K, group, x, "linear4: payload must be contiguous uint32 [N, 4 * ceil(K / 32)] and scale float16 [N, ceil(K / group)] on x's device");
+    require(!residual.defined() || (residual.device() == x.device() && residual.numel() == T * N), "linear4: residual must be [T, N] on x's device");
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (residual.defined()) residual = contiguous(residual.scalar_type() == x.scalar_type() ? residual : residual.to(x.scalar_type()));
+    const at::Tensor y = at::empty({T, N}, x.options());
+    check(bm_linear4(x.data_ptr(), dtype, static_cast<const uint32_t*>(p.data_ptr()), wptr(s), static_cast<int32_t>(T), static_cast<int32_t>(K),
+                     static_cast<int32_t>(N), group, ptr(residual), y.data_ptr(), stream_of(x.device())));
+    return THPVariable_Wrap(y);
+  });
+}
+
+// (x [T, H], gate payload, scale, up payload, scale, down payload, scale, group size, token gate | None, residual | None) -> y [T, H]
+PyObject* dense_mlp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 10);
+    const at::Tensor x = contiguous(tensor(a[0])), &gp = tensor(a[1]), &gs = tensor(a[2]), &up = tensor(a[3]), &us = tensor(a[4]), &dp = tensor(a[5]), &ds = tensor(a[6]);
+    const int32_t group = group_size(a[7]);
+    at::Tensor tg = opt_tensor(a[8]), residual = opt_tensor(a[9]);
+    require_cuda(x, "dense_mlp4");
+    refuse_grad("dense_mlp4", {&x, &gs, &us, &ds, &tg, &residual});
+    const int dtype = half_code(x, "dense_mlp4: x must be float16 or bfloat16");
+    require(x.dim() == 2 && x.size(1) > 0 && gp.dim() == 2 && gp.size(0) > 0, "dense_mlp4: x must be [T, H] and the gate matrix have rows");
+    const int64_t T = x.size(0), H = x.size(1), I = gp.size(0);
+    for (int64_t v : {T, H, I}) require_int32_range(v, "dense_mlp4: a size exceeds 32 bits");
+    require_matrix4(gp, gs, I, H, group, x, "dense_mlp4: the gate matrix must be packed [intermediate, hidden] on x's device");
+    require_matrix4(up, us, I, H, group, x, "dense_mlp4: the up matrix must be packed [intermediate, hidden] on x's device");
+    require_matrix4(dp, ds, H, I, group, x, "dense_mlp4: the down matrix must be packed [hidden, intermediate] on x's device");
+    require(!tg.defined() || (tg.numel() == H && tg.device() == x.device()), "dense_mlp4: the token gate's weight must have hidden elements on x's device");
+    require_residual(residual, x);
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (tg.defined()) tg = contiguous(tg.scalar_type() == at::kHalf ? tg : tg.to(at::kHalf));
+    if (residual.defined()) residual = contiguous(residual.scalar_type() == x.scalar_type() ? residual : residual.to(x.scalar_type()));
+    const at::Tensor y = at::empty_like(x);
+    const at::Tensor ws = scratch(bm_dense_mlp4_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(I)), x);
+    auto words = [](const at::Tensor& t) { return static_cast<const uint32_t*>(t.data_ptr()); };
+    check(bm_dense_mlp4_forward(x.data_ptr(), dtype, words(gp), wptr(gs), words(up), wptr(us), words(dp), wptr(ds), wptr(tg), static_cast<int32_t>(T),
+                                static_cast<int32_t>(H), static_cast<int32_t>(I), group, ptr(residual), y.data_ptr(), ws.data_ptr(), ws.nbytes(),
+                                stream_of(x.device())));
+    return THPVariable_Wrap(y);
+  });
+}
+
 at::Tensor run_experts(HostLayer* L, const at::Tensor& hg, const at::Tensor& hu, const at::Tensor& tok, const at::Tensor& off,
                        const at::Tensor& rw, int64_t rank_out, int32_t path) {
   // h_up may have fewer rows than h_gate: only the rows that token_indices names are read
@@ -602,7 +671,7 @@ PyObject* pack_matrix(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(layer_new), FAST(layer_close), FAST(layer_drop_workspaces), FAST(layer_workspace), FAST(layer_forward),
-                         FAST(block_forward), FAST(dense_mlp), FAST(grouped_linear), FAST(dense_experts), FAST(experts_forward), FAST(op_forward), FAST(op_register), FAST(pack_matrix),
+                         FAST(block_forward), FAST(dense_mlp), FAST(grouped_linear), FAST(dense_experts), FAST(linear4), FAST(dense_mlp4), FAST(experts_forward), FAST(op_forward), FAST(op_register), FAST(pack_matrix),
                          {"op_clear", op_clear, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bm_host", "Native host path of bitsmoe_b200.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,379 @@
+// Products with 4-bit weights and one fp16 scale for every 32, 64 or 128 columns of a row:
+//   y[t][n] = sum_k x[t][k] * scale[n][k / group] * (code[n][k] - 8)   (+ residual[t][n])
+// The code of column 8 j + i is in bits 4 i .. 4 i + 3 of word j of the row; rows are padded to whole 16 bytes.
+//
+// linear4_kernel streams the weights once per 32 tokens.  A warp takes 16 rows; lane (g, t) of it holds, for rows g and g + 8, the words of
+// group / 4 neighbouring columns, so that one mma.sync m16n8k16 never crosses a group: contraction position is whatever order both
+// operands agree on, and x is put into that order once per CTA (shared memory, 16 bytes per lane and word).  Codes become exact
+// 16-bit numbers -8 .. 7 of x's type by mask and subtraction of a constant; products of a group are summed in fp32 by the tensor
+// core and multiplied by the group's scale in fp32, so nothing but the output is rounded.  Few rows: the eight warps of a CTA and the
+// CTAs of a cluster share a row's columns and meet in shared memory, in a fixed order.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "grouped.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace bm {
+
+int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st);
+
+constexpr int L4_THREADS = 256, L4_WARPS = 8, L4_CHUNK = 128, L4_BATCH = 4;
+constexpr size_t L4_SMEM = 110 * 1024;          // two CTAs an SM
+
+struct Linear4Args {
+  const uint32_t* p[2];        // codes [N, words]; GLU: gate and up
+  const __half* s[2];          // scales [N, groups]
+  const void* x;               // [T, ldx]
+  const void* residual;        // [T, N] of y's type, or null
+  const float* row_gate;       // factor per token, or null
+  void* y;                     // [T, ldy]
+  int T, K, N, ldx, ldy, words, groups;
+  int glu, y_dtype, vec_x, kwarps, splits, row_blocks;
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight codes -> four pairs (code i, code i + 4), i = 0 .. 3, as exact numbers -8 .. 7 of the type.
+template <int XD>
+__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&q)[4]) {
+  if (XD == BM_F16) {
+    // 1024 + u and 1024 + 16 u are fp16 numbers with u in their low mantissa bits
+    const __half2 off = __float2half2_rn(1032.f), sixteenth = __float2half2_rn(0.0625f), minus72 = __float2half2_rn(-72.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h, w >>= 8) {
+      const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x64006400u;
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off), b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, minus72);
+      q[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
+      q[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  } else {
+    const __nv_bfloat162 off = __float2bfloat162_rn(136.f);       // 128 + u
+#pragma unroll
+    for (int i = 0; i < 4; ++i, w >>= 4) {
+      const uint32_t v = (w & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+      q[i] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+  }
+}
+
+// Place of word kw (eight columns of x) among the words of a CTA: the words that a quad's lanes use together are neighbours.
+template <int WPL>
+__device__ __forceinline__ int l4_place(int kw) { return (kw / (4 * WPL)) * (4 * WPL) + (kw % WPL) * 4 + (kw / WPL) % 4; }
+// Byte offset of token n's piece: NT pieces of 16 bytes a word, swapped so that eight neighbouring lanes (two tokens, four words) hit
+// eight different bank groups.
+template <int NT>
+__device__ __forceinline__ int l4_piece(int place, int n) {
+  const int t = place & 3, sw = NT >= 8 ? 2 * t : 0;
+  return (place * NT + (n ^ sw)) * 16;
+}
+
+template <int NT, int XD, int WPL>
+__global__ void __launch_bounds__(L4_THREADS, 2) linear4_kernel(const __grid_constant__ Linear4Args a) {
+  constexpr int NB = NT < 8 ? 1 : NT / 8, GPC = 4 / WPL, SPR = (L4_BATCH * GPC + 3) / 4;     // groups a chunk, scale loads per row and batch
+  extern __shared__ __align__(16) unsigned char l4_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % a.splits, kw = warp % a.kwarps, rw = warp / a.kwarps, rws = L4_WARPS / a.kwarps;
+  const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK;
+  const int c_first = chunks * split / a.splits, c_end = chunks * (split + 1) / a.splits;           // this CTA's chunks of 128 columns
+  const int n0 = blockIdx.y * NT, nn = min(NT, a.T - n0);
+  float* const recv = reinterpret_cast<float*>(l4_smem + static_cast<size_t>((chunks + a.splits - 1) / a.splits) * (L4_CHUNK / 8) * NT * 16);
+  grid_launch_dependents();
+  grid_wait();
+  // ---- x of this CTA's columns, in the order of the products
+  {
+    const int words = (c_end - c_first) * (L4_CHUNK / 8);
+    for (int i = threadIdx.x; i < words * nn; i += L4_THREADS) {
+      const int n = i / words, w = i - n * words, k = c_first * L4_CHUNK + 8 * w;
+      const uint16_t* src = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(n0 + n) * a.ldx + k;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (a.vec_x && k + 8 <= a.K) v = *reinterpret_cast<const uint4*>(src);
+      else {
+        uint16_t* e = reinterpret_cast<uint16_t*>(&v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k + j < a.K) e[j] = src[j];
+      }
+      *reinterpret_cast<uint4*>(l4_smem + l4_piece<NT>(l4_place<WPL>(w), n)) =
+          make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+    }
+  }
+  __syncthreads();
+  const int wc = c_end - c_first, w_first = wc * kw / a.kwarps, w_end = wc * (kw + 1) / a.kwarps;      // this warp's chunks, CTA-relative
+  const int per = a.glu ? 8 : 16, cluster_id = blockIdx.x / a.splits, clusters = gridDim.x / a.splits;
+  for (int rb = cluster_id; rb < a.row_blocks; rb += clusters) {
+    const int r0 = (rb * rws + rw) * per;
+    // rows g and g + 8 of the unit
+    const int ra = r0 + g, rc = a.glu ? ra : r0 + 8 + g;
+    const uint32_t* pa = a.p[0] + static_cast<int64_t>(min(ra, a.N - 1)) * a.words;
+    const uint32_t* pc = (a.glu ? a.p[1] : a.p[0]) + static_cast<int64_t>(min(rc, a.N - 1)) * a.words;
+    const __half* sa = a.s[0] + static_cast<int64_t>(min(ra, a.N - 1)) * a.groups;
+    const __half* sc = (a.glu ? a.s[1] : a.s[0]) + static_cast<int64_t>(min(rc, a.N - 1)) * a.groups;
+    float acc[NB][4] = {};
+    uint32_t w[2][2][L4_BATCH][4];           // [buffer][row][chunk][word]
+    float sv[2][2][SPR];                     // lane t: scale of group 4 i + t of the batch
+    auto fetch = [&](int c, uint32_t (&wd)[2][L4_BATCH][4], float (&sd)[2][SPR]) {
+#pragma unroll
+      for (int u = 0; u < L4_BATCH; ++u) {
+        const int word = (c_first + c + u) * (L4_CHUNK / 8);
+#pragma unroll
+        for (int j = 0; j < GPC; ++j) {
+          const int at = word + (j * 4 + t) * WPL;
+          const bool in = c + u < w_end && at < a.words;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t* src = (r ? pc : pa) + at;
+            if (WPL == 4) {
+              const uint4 v = in ? __ldcs(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
+              wd[r][u][0] = v.x; wd[r][u][1] = v.y; wd[r][u][2] = v.z; wd[r][u][3] = v.w;
+            } else if (WPL == 2) {
+              const uint2 v = in ? __ldcs(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
+              wd[r][u][2 * j] = v.x; wd[r][u][2 * j + 1] = v.y;
+            } else {
+              wd[r][u][j] = in ? __ldg(src) : 0u;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < SPR; ++i) {
+        const int grp = (c_first + c) * GPC + 4 * i + t;
+        const bool in = grp < a.groups && c + (4 * i + t) / GPC < w_end;
+        sd[0][i] = in ? __half2float(sa[grp]) : 0.f;
+        sd[1][i] = in ? __half2float(sc[grp]) : 0.f;
+      }
+    };
+    auto multiply = [&](int c, const uint32_t (&wd)[2][L4_BATCH][4], const float (&sd)[2][SPR]) {
+#pragma unroll
+      for (int u = 0; u < L4_BATCH; ++u) {
+        if (c + u >= w_end) break;
+#pragma unroll
+        for (int j = 0; j < GPC; ++j) {
+          float part[NB][4] = {};
+#pragma unroll
+          for (int v = 0; v < WPL; ++v) {
+            uint32_t qa[4], qc[4];
+            codes_to_pairs<XD>(wd[0][u][j * WPL + v], qa);
+            codes_to_pairs<XD>(wd[1][u][j * WPL + v], qc);
+            const uint32_t first[4] = {qa[0], qc[0], qa[1], qc[1]}, second[4] = {qa[2], qc[2], qa[3], qc[3]};
+            const int place = (c + u) * (L4_CHUNK / 8) + (j * WPL + v) * 4 + t;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const int n = 8 * b + g;
+              uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+              if (n < nn) xv = *reinterpret_cast<const uint4*>(l4_smem + l4_piece<NT>(place, n));
+              if (XD == BM_F16) {
+                mma_f16_16816(part[b], first, xv.x, xv.y);
+                mma_f16_16816(part[b], second, xv.z, xv.w);
+              } else {
+                mma_bf16_16816(part[b], first, xv.x, xv.y);
+                mma_bf16_16816(part[b], second, xv.z, xv.w);
+              }
+            }
+          }
+          const int q = u * GPC + j;
+          const float f0 = __shfl_sync(0xffffffffu, sd[0][q / 4], (lane & ~3) + q % 4), f1 = __shfl_sync(0xffffffffu, sd[1][q / 4], (lane & ~3) + q % 4);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            acc[b][0] = fmaf(part[b][0], f0, acc[b][0]);
+            acc[b][1] = fmaf(part[b][1], f0, acc[b][1]);
+            acc[b][2] = fmaf(part[b][2], f1, acc[b][2]);
+            acc[b][3] = fmaf(part[b][3], f1, acc[b][3]);
+          }
+        }
+      }
+    };
+    fetch(w_first, w[0], sv[0]);
+    for (int c = w_first; c < w_end; c += 2 * L4_BATCH) {
+      if (c + L4_BATCH < w_end) fetch(c + L4_BATCH, w[1], sv[1]);
+      multiply(c, w[0], sv[0]);
+      if (c + L4_BATCH >= w_end) break;
+      if (c + 2 * L4_BATCH < w_end) fetch(c + 2 * L4_BATCH, w[0], sv[0]);
+      multiply(c + L4_BATCH, w[1], sv[1]);
+    }
+    // ---- sums of the warps (and CTAs) that share the rows, then out
+    auto finish = [&](int row, int n, float v) {
+      const int64_t o = static_cast<int64_t>(n0 + n) * a.ldy + row;
+      if (a.row_gate) v *= a.row_gate[n0 + n];
+      if (a.residual) v += load_act(a.residual, a.y_dtype, static_cast<int64_t>(n0 + n) * a.N + row);
+      store_act(a.y, a.y_dtype, o, v);
+    };
+    if (a.kwarps == 1 && a.splits == 1) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = 8 * b + 2 * t + i;
+          if (n >= nn) continue;
+          if (a.glu) {
+            if (ra < a.N) finish(ra, n, silu_mul(acc[b][i], acc[b][2 + i]));
+          } else {
+            if (ra < a.N) finish(ra, n, acc[b][i]);
+            if (rc < a.N) finish(rc, n, acc[b][2 + i]);
+          }
+        }
+      continue;
+    }
+    constexpr int COLS = 8 * NB, PART = 16 * COLS;       // floats of one warp's part: [row][token]
+    float* mine = recv + (split * L4_WARPS + warp) * PART;
+    if (a.splits > 1) {
+      cg::this_cluster().sync();                         // the first CTA runs, and has read the parts of the rows before
+      mine = cg::this_cluster().map_shared_rank(mine, 0);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      *reinterpret_cast<float2*>(mine + g * COLS + 8 * b + 2 * t) = make_float2(acc[b][0], acc[b][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * COLS + 8 * b + 2 * t) = make_float2(acc[b][2], acc[b][3]);
+    }
+    if (a.splits > 1) cg::this_cluster().sync();
+    else __syncthreads();
+    if (split == 0) {
+      const int outs = per * rws;
+      for (int o = threadIdx.x; o < outs * nn; o += L4_THREADS) {
+        const int n = o / outs, r = o - n * outs, wr = r / per, row = r - wr * per, out_row = (rb * rws + wr) * per + row;
+        if (out_row >= a.N) continue;
+        float v = 0.f, u = 0.f;
+        for (int s = 0; s < a.splits; ++s)
+          for (int k = 0; k < a.kwarps; ++k) {
+            const float* part = recv + (s * L4_WARPS + wr * a.kwarps + k) * PART + n;
+            v += part[row * COLS];
+            if (a.glu) u += part[(row + 8) * COLS];
+          }
+        finish(out_row, n, a.glu ? silu_mul(v, u) : v);
+      }
+    }
+    if (a.splits == 1) __syncthreads();                  // the parts may be overwritten
+  }
+}
+
+static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
+  const int chunks = (K + L4_CHUNK - 1) / L4_CHUNK, cols = nt < 8 ? 8 : nt;
+  return static_cast<size_t>((chunks + splits - 1) / splits) * (L4_CHUNK / 8) * nt * 16 + (shared_rows ? static_cast<size_t>(splits) * L4_WARPS * 16 * cols * 4 : 0);
+}
+
+template <int NT, int XD, int WPL>
+static int l4_launch_one(const Linear4Args& a, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
+  static PerDeviceOnce once;
+  int dev = -1;
+  BM_CUDA(cudaGetDevice(&dev));
+  if (!once.is_done(dev)) {
+    BM_CUDA(cudaFuncSetAttribute(linear4_kernel<NT, XD, WPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    once.mark(dev);
+  }
+  BM_CUDA(launch_after(after, a.splits, linear4_kernel<NT, XD, WPL>, grid, L4_THREADS, smem, st, a));
+  BM_LAUNCH_CHECK("linear4_kernel");
+  return BM_OK;
+}
+template <int NT, int XD>
+static int l4_launch_group(const Linear4Args& a, int group, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
+  return group == 128 ? l4_launch_one<NT, XD, 4>(a, grid, smem, after, st) : group == 64 ? l4_launch_one<NT, XD, 2>(a, grid, smem, after, st)
+                                                                                       : l4_launch_one<NT, XD, 1>(a, grid, smem, after, st);
+}
+template <int NT>
+static int l4_launch(const Linear4Args& a, int x_dtype, int group, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
+  return x_dtype == BM_F16 ? l4_launch_group<NT, BM_F16>(a, group, grid, smem, after, st) : l4_launch_group<NT, BM_BF16>(a, group, grid, smem, after, st);
+}
+
+// y = x . W^T, or with glu z = silu(x . Wg^T) * (x . Wu^T).
+static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cudaStream_t st) {
+  a.words = (a.K + 31) / 32 * 4;
+  a.groups = (a.K + group - 1) / group;
+  a.vec_x = aligned16(a.x) && a.ldx % 8 == 0;
+  const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK, units = (a.N + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
+  int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32;
+  // warps of a CTA, then CTAs of a cluster, share a row's columns until every SM has work
+  a.kwarps = 1; a.splits = 1;
+  while (a.kwarps < 8 && a.kwarps < chunks && units * a.kwarps < 148 * 16) a.kwarps *= 2;
+  while (nt > 8 && l4_smem_bytes(nt, a.K, 8, true) > 200 * 1024) nt /= 2;
+  while (a.splits < 8 && l4_smem_bytes(nt, a.K, a.splits, true) > L4_SMEM) a.splits *= 2;
+  BM_REQUIRE(l4_smem_bytes(nt, a.K, a.splits, true) <= 220 * 1024, BM_ERR_UNSUPPORTED, "linear4: %d columns are too many", a.K);
+  const int rws = L4_WARPS / a.kwarps;
+  a.row_blocks = (units + rws - 1) / rws;
+  const int most = 148 * 2 / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
+  const dim3 g(grid, (a.T + nt - 1) / nt);
+  const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
+  switch (nt) {
+    case 2: return l4_launch<2>(a, x_dtype, group, g, smem, after, st);
+    case 8: return l4_launch<8>(a, x_dtype, group, g, smem, after, st);
+    case 16: return l4_launch<16>(a, x_dtype, group, g, smem, after, st);
+    default: return l4_launch<32>(a, x_dtype, group, g, smem, after, st);
+  }
+}
+
+}  // namespace bm
+
+using namespace bm;
+
+static int l4_check(const char* what, int dtype, int32_t T, int32_t group, std::initializer_list<int32_t> sizes) {
+  BM_REQUIRE(T >= 0, BM_ERR_INVALID_ARG, "%s: bad sizes", what);
+  for (int32_t v : sizes) {
+    BM_REQUIRE(v > 0, BM_ERR_INVALID_ARG, "%s: bad sizes", what);
+    BM_REQUIRE(v < (1 << 30), BM_ERR_UNSUPPORTED, "%s: size %d is too large", what, v);
+  }
+  BM_REQUIRE(dtype == BM_F16 || dtype == BM_BF16, BM_ERR_INVALID_ARG, "%s: x must be fp16 or bf16", what);
+  BM_REQUIRE(group == 32 || group == 64 || group == 128, BM_ERR_UNSUPPORTED, "%s: groups of %d columns; 32, 64 and 128 are supported", what, group);
+  return BM_OK;
+}
+
+extern "C" int bm_linear4(const void* x, int dtype, const uint32_t* payload, const uint16_t* scale, int32_t T, int32_t K, int32_t N, int32_t group,
+                          const void* residual, void* y, void* stream) {
+  bm::NvtxRange nvtx_range("bm_linear4");
+  const int rc = l4_check("linear4", dtype, T, group, {K, N});
+  if (rc) return rc;
+  if (T == 0) return BM_OK;
+  BM_REQUIRE(x && payload && scale && y, BM_ERR_INVALID_ARG, "linear4: null pointer");
+  BM_REQUIRE(aligned16(payload), BM_ERR_INVALID_ARG, "linear4: the codes must start on a 16-byte boundary");
+  Linear4Args a{};
+  a.p[0] = payload; a.s[0] = reinterpret_cast<const __half*>(scale);
+  a.x = x; a.residual = residual; a.y = y;
+  a.T = T; a.K = K; a.N = N; a.ldx = K; a.ldy = N; a.y_dtype = dtype;
+  return linear4(a, dtype, group, AFTER_ALL, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t bm_dense_mlp4_workspace_bytes(int32_t T, int32_t intermediate) {
+  if (T <= 0 || intermediate <= 0) return 0;
+  // z [T, intermediate], rows of whole 16 bytes, and the per-token gate
+  return align_up(static_cast<size_t>(T) * align_up(intermediate, 8) * 2, 256) + align_up(static_cast<size_t>(T) * 4, 256);
+}
+
+extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* gate_payload, const uint16_t* gate_scale, const uint32_t* up_payload,
+                                     const uint16_t* up_scale, const uint32_t* down_payload, const uint16_t* down_scale, const uint16_t* token_gate_w,
+                                     int32_t T, int32_t hidden, int32_t intermediate, int32_t group, const void* residual, void* y, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  bm::NvtxRange nvtx_range("bm_dense_mlp4_forward");
+  int rc = l4_check("dense_mlp4", dtype, T, group, {hidden, intermediate});
+  if (rc) return rc;
+  if (T == 0) return BM_OK;
+  BM_REQUIRE(x && gate_payload && gate_scale && up_payload && up_scale && down_payload && down_scale && y, BM_ERR_INVALID_ARG, "dense_mlp4: null pointer");
+  BM_REQUIRE(aligned16(gate_payload, up_payload, down_payload), BM_ERR_INVALID_ARG, "dense_mlp4: the codes must start on a 16-byte boundary");
+  const size_t need = bm_dense_mlp4_workspace_bytes(T, intermediate);
+  BM_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, BM_ERR_WORKSPACE,
+             "dense_mlp4: workspace must be 256-byte aligned and hold %zu bytes (%zu given)", need, workspace_bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int ldz = static_cast<int>(align_up(intermediate, 8));
+  void* z = workspace;
+  float* gate = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align_up(static_cast<size_t>(T) * ldz * 2, 256));
+  if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_ALL, st))) return rc;
+  Linear4Args a{};
+  a.p[0] = gate_payload; a.p[1] = up_payload;
+  a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
+  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.y_dtype = dtype; a.glu = 1;
+  if ((rc = linear4(a, dtype, group, token_gate_w ? AFTER_READS : AFTER_ALL, st))) return rc;
+  Linear4Args d{};
+  d.p[0] = down_payload; d.s[0] = reinterpret_cast<const __half*>(down_scale);
+  d.x = z; d.residual = residual; d.row_gate = token_gate_w ? gate : nullptr; d.y = y;
+  d.T = T; d.K = intermediate; d.N = hidden; d.ldx = ldz; d.ldy = hidden; d.y_dtype = dtype;
+  return linear4(d, dtype, group, AFTER_READS, st);
+}

@@ -316,3 +316,22 @@ def dense_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
     if not x.is_cuda:
         raise RuntimeError("dense_experts requires CUDA tensors; there is no CPU path")
     return capi.host().dense_experts(x, topk_idx, topk_w, w_gate_up, w_down, global_to_local, residual)
+
+
+def linear4(x: torch.Tensor, payload: torch.Tensor, scale: torch.Tensor, group_size: int = 128,
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ W.T (+ ``residual``) with W in 4 bits: (payload, scale) as ``quant.linear4.quantize_linear4`` makes them.  x [T, K] fp16 or
+    bf16 -> [T, N] of x's type.  Codes and x enter the products unrounded, sums and scales are fp32; forward only."""
+    if not x.is_cuda:
+        raise RuntimeError("linear4 requires CUDA tensors; there is no CPU path")
+    return capi.host().linear4(x, payload, scale, group_size, residual)
+
+
+def dense_mlp4(x: torch.Tensor, gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, torch.Tensor],
+               down: Tuple[torch.Tensor, torch.Tensor], group_size: int = 128, token_gate_weight: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dense_mlp`` with its three matrices in 4 bits, each a (payload, scale) pair of ``quant.linear4``: (silu(x Wg^T) * (x Wu^T))
+    Wd^T, scaled per token by sigmoid(x . token_gate_weight) when that is given, plus ``residual``.  x [T, H] fp16 or bf16."""
+    if not x.is_cuda:
+        raise RuntimeError("dense_mlp4 requires CUDA tensors; there is no CPU path")
+    return capi.host().dense_mlp4(x, *gate, *up, *down, group_size, None if token_gate_weight is None else token_gate_weight.reshape(-1), residual)

@@ -273,6 +273,22 @@ BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* top
                                     const void* w_down, int32_t hidden, int32_t intermediate, const void* residual, void* y,
                                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- products with 4-bit weights ------------------------------------------
+ * y[t][n] = sum_k x[t][k] * scale[n][k / group] * (code[n][k] - 8) (+ residual): x [T, K], residual (may be NULL) and y [T, N] of
+ * `dtype` (fp16 or bf16).  payload uint32 [N, 4 * ceil(K / 32)], 16-byte aligned: the code of column 8 j + i in bits 4 i .. 4 i + 3 of
+ * word j of its row; codes behind column K are not used.  scale fp16 [N, ceil(K / group)], group 32, 64 or 128.  Codes and x enter the
+ * products as they are, sums and scales are fp32: only y is rounded. */
+BM_API int bm_linear4(const void* x, int dtype, const uint32_t* payload, const uint16_t* scale, int32_t T, int32_t K, int32_t N,
+                      int32_t group, const void* residual, void* y, void* stream);
+/* SwiGLU MLP with such weights, as bm_dense_mlp_forward: y = f * (silu(x . Wg^T) * (x . Wu^T)) . Wd^T (+ residual), f = 1 or, with
+ * token_gate_w (fp16 [hidden]), sigmoid(x . token_gate_w).  gate and up [intermediate, hidden], down [hidden, intermediate]; the value
+ * between the products is held in `dtype`. */
+BM_API size_t bm_dense_mlp4_workspace_bytes(int32_t T, int32_t intermediate);
+BM_API int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* gate_payload, const uint16_t* gate_scale,
+                                 const uint32_t* up_payload, const uint16_t* up_scale, const uint32_t* down_payload,
+                                 const uint16_t* down_scale, const uint16_t* token_gate_w, int32_t T, int32_t hidden, int32_t intermediate,
+                                 int32_t group, const void* residual, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- whole block -------------------------------------------------------
  * The dense parts of a block beside its packed experts, in the model's own type (w_dtype: BM_F16, or BM_BF16, which is
  * rounded to fp16 on the way to the tensor cores); pointers that are NULL are left out.  `gate_w` [num_routed, hidden] is
