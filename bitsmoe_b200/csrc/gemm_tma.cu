@@ -496,6 +496,14 @@ static bool make_map(CUtensorMap* map, const void* base, int rows, int cols, int
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 16-bit elements, `rank` dimensions from the innermost (contiguous) one, 128-byte rows with the 128-byte swizzle; false when it cannot be described.
+bool encode_map16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BN, int XD, int SPLIT>
 static int launch_one(const GtParams& p, LaunchAfter after, int grid, cudaStream_t st) {
   const int smem = gt_stages(BN, XD, SPLIT) * gt_stage_bytes(BN, XD) + gt_tail_bytes(BN, SPLIT) + 1024;

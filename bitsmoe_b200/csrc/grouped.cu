@@ -95,6 +95,8 @@ __global__ void __launch_bounds__(GG_THREADS) grouped_any_kernel(const GroupedAr
 
 int launch_grouped(const GroupedArgs& a, cudaStream_t st) {
   if (a.rows == 0 || a.E == 0) return BM_OK;
+  const int rc = launch_grouped_tc(a, st);
+  if (rc != BM_ERR_UNSUPPORTED) return rc;
   const int64_t tiles = a.rows / GG_ROWS + static_cast<int64_t>(a.E < a.rows ? a.E : a.rows) + 1;
   const dim3 grid((a.N + GG_COLS - 1) / GG_COLS, static_cast<unsigned>(tiles < 65535 ? tiles : 65535));
   auto* kernel = a.dtype == BM_F16 ? (a.glu ? grouped_any_kernel<BM_F16, true> : grouped_any_kernel<BM_F16, false>)

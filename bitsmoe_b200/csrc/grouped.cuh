@@ -29,6 +29,9 @@ __device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int ro
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
+// BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies (grouped_tc.cu).
+int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st);
+// The tensor-core kernel, else the one that takes every shape.
 int launch_grouped(const GroupedArgs& a, cudaStream_t st);
 
 }  // namespace bm

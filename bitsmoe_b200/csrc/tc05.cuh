@@ -98,6 +98,8 @@ __device__ __forceinline__ uint64_t smem_desc_kmajor(uint32_t saddr, uint32_t lb
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t M, uint32_t N) {
   return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
+// the same for bf16 x bf16
+__host__ __device__ constexpr uint32_t idesc_bf16(uint32_t M, uint32_t N) { return idesc_f16(M, N) | (1u << 7) | (1u << 10); }
 
 // D[tmem] (+)= A[smem] * B[smem]^T, issued by one thread
 __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
