@@ -17,6 +17,8 @@ struct GroupedArgs {
   int x_rows, rows, K, N, E;
   int dtype, y_dtype;          // of x and w: BM_F16 or BM_BF16; of y: the same or BM_F32
   int glu;
+  int expected;                // rows that the groups are expected to have, 0 = `rows`
+  void* gathered;              // with an index: room for [rows, K], 16-byte aligned, or null
   LaunchAfter after;
 };
 
@@ -31,6 +33,8 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 
 // BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies (grouped_tc.cu).
 int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st);
+// Whether rows picked by an index are brought into expert order before the products.
+bool grouped_gathers(int expected, int E, int K);
 // The tensor-core kernel, else the one that takes every shape.
 int launch_grouped(const GroupedArgs& a, cudaStream_t st);
 

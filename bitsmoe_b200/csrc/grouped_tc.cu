@@ -5,12 +5,12 @@
 // (expert, up to 256 of its rows, 256 weight rows): each CTA loads 128 weight rows and half of the item's rows, and the tensor cores
 // read both halves, so that an SM fetches 32 KB per 64 columns of K for 128 x 256 sums (a lone CTA would need 48, which is more than an SM gets
 // from L2 while its tensor core multiplies them).
-//   warp 0      producer: weight rows as tiled copies, the rows of x by tile::gather4 (a lane names four of them), all onto the even CTA's barrier
+//   warp 0      producer: weight rows and rows of x as tiled copies, or rows of x by tile::gather4 (a lane names four of them), all onto
+//               the even CTA's barrier
 //   warp 1      MMA issue, in the even CTA for both: four tcgen05.mma (M = 256, N = the item's rows, K = 16) per stage
-//   warps 4-11  epilogue: tensor memory -> registers -> y.  A lane owns an output column (weight row), so that a warp's store is one
-//               contiguous piece of a row of y and needs no alignment.  With a gated pair a quarter of the accumulator's lanes holds
-//               16 gate rows and the 16 up rows that belong to them; lanes l and l + 16 exchange every other row's sums and each
-//               finishes one of two rows.
+//   warps 4-11  epilogue: tensor memory -> registers (fragments of 16 weight rows x 8 rows) -> y.  stmatrix turns them round in
+//               shared memory, so that a thread stores 16 bytes of a row of y.  With a gated pair the accumulator's lanes alternate between
+//               16 gate rows and the 16 up rows that belong to them, so that a thread holds both sums of an output.
 // The accumulator alternates between two halves of tensor memory.  Items are handed out round robin; which expert an item belongs
 // to every CTA works out from the offsets, so that the host never reads them.  Waits are bounded.
 #include <cuda.h>
@@ -24,25 +24,34 @@ namespace bm {
 
 bool encode_map16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 
-constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_STAGES = 6, GC_MAX_E = 1024;
-constexpr int GC_A_BYTES = 128 * GC_K * 2, GC_B_BYTES = 128 * GC_K * 2, GC_STAGE = GC_A_BYTES + GC_B_BYTES;
-constexpr int gc_smem_bytes(int E) { return GC_STAGES * GC_STAGE + 1024 + (3 * E + 1) * 4; }
+constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_MAX_STAGES = 12, GC_MAX_E = 1024;
+constexpr int GC_TURN_PITCH = 80, GC_TURN_BYTES = 32 * GC_TURN_PITCH;      // 32 rows of 64 (gated pair: 32) bytes: eight rows hit eight bank groups
+constexpr int GC_A_BYTES = 128 * GC_K * 2, GC_BOX = 32;
+// The ring: stages of 128 weight rows and half of the rows of the longest item that the offsets make, 6 of 32 KB to 11 of 17 KB.
+constexpr int GC_RING = 6 * 2 * GC_A_BYTES;
+constexpr int gc_smem_bytes(int E) { return GC_RING + GC_EPI_WARPS * GC_TURN_BYTES + 1024 + (3 * E + 1) * 4; }
 
 struct GcParams {
-  CUtensorMap x, w;
+  CUtensorMap x, x8, w;        // x: 32 rows in order (one row of a gather), or 8
   const int32_t* offsets;
   const int32_t* index;
   void* y;
-  int x_rows, rows, N, E, slices, blocks, y_dtype, bf16;     // blocks: items along the weight rows
+  int x_rows, rows, N, E, slices, blocks, vec;     // blocks: items along the weight rows; vec: y takes 16-byte stores
 };
 
-// 2-D gather of four rows / 3-D and 4-D tiles into this CTA's shared memory, signalled on `bar` (shared::cluster address)
+// Copies into this CTA's shared memory, signalled on `bar` (shared::cluster address, of either CTA of the pair): four rows, tiles.
 __device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* map, int x, int4 r, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
           tc::smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
       : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -65,13 +74,17 @@ __device__ __forceinline__ uint64_t gc_desc(uint32_t saddr) {
 struct GcTable {
   const int *first, *start, *count;     // [E + 1] items before the group; its first row; its rows
 };
+// Rows of the pieces of a group of n rows, a multiple of 16 (a lesser last one apart).
+__device__ __forceinline__ int gc_piece(int n) {
+  const int pieces = (n + GC_ROWS - 1) / GC_ROWS;
+  return pieces ? ((n + pieces - 1) / pieces + 15) & ~15 : 0;
+}
 struct GcItem {
   int e, row0, rows, block;
 };
 __device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int blocks, int& e) {
   while (item >= tab.first[e + 1]) ++e;
-  const int local = item - tab.first[e], piece = local / blocks, n = tab.count[e], pieces = (n + GC_ROWS - 1) / GC_ROWS;
-  const int size = ((n + pieces - 1) / pieces + 15) & ~15;
+  const int local = item - tab.first[e], piece = local / blocks, n = tab.count[e], size = gc_piece(n);
   GcItem it;
   it.e = e;
   it.block = local - piece * blocks;
@@ -80,18 +93,35 @@ __device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int bloc
   return it;
 }
 
-template <bool GLU>
+template <bool BF16>
+__device__ __forceinline__ uint32_t gc_pack(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four 8 x 8 fragments, turned round: lane 8 m + j names the 16 bytes that column j of fragment m goes to.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// F32: y is fp32 (no gated pair).  GATHER: rows of x by index.
+template <bool GLU, bool GATHER, bool F32, bool BF16>
 __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_constant__ GcParams p) {
   extern __shared__ unsigned char gc_raw[];
-  __shared__ __align__(8) uint64_t full[GC_STAGES], empty[GC_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[GC_MAX_STAGES], empty[GC_MAX_STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ int longest;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gc_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  int* const t_first = reinterpret_cast<int*>(smem + GC_STAGES * GC_STAGE);
+  unsigned char* const turn = smem + GC_RING;
+  int* const t_first = reinterpret_cast<int*>(turn + GC_EPI_WARPS * GC_TURN_BYTES);
   int *const t_start = t_first + p.E + 1, *const t_count = t_start + p.E;
   const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < GC_STAGES; ++i) {
+    for (int i = 0; i < GC_MAX_STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
@@ -117,10 +147,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   tc::fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   if (warp == 0) {
-    int before = 0;
+    int before = 0, most = 16;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane;
-      int incl = e < p.E ? (t_count[e] + GC_ROWS - 1) / GC_ROWS * p.blocks : 0;
+      const int e = e0 + lane, n = e < p.E ? t_count[e] : 0;
+      most = max(most, gc_piece(n));
+      int incl = (n + GC_ROWS - 1) / GC_ROWS * p.blocks;
       const int mine = incl;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -130,11 +161,16 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (e < p.E) t_first[e] = before + incl - mine;
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) t_first[p.E] = before;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      t_first[p.E] = before;
+      longest = most;
+    }
   }
   __syncthreads();
   const GcTable tab{t_first, t_start, t_count};
   const int items = t_first[p.E], pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int stage = GC_A_BYTES + longest / 2 * GC_K * 2, stages = min(GC_RING / stage, GC_MAX_STAGES);
   bool ok = true;
 
   if (warp == 0) {
@@ -143,20 +179,21 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs) {
       const GcItem it = gc_item(tab, item, p.blocks, e);
-      const int half = ((it.rows + 15) & ~15) >> 1;
-      int4 src;
-      int* s = reinterpret_cast<int*>(&src);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // columns past the item's rows are not used: they repeat its last row
-        const int r = it.row0 + min(static_cast<int>(rank) * half + 4 * lane + j, it.rows - 1);
-        const int id = p.index ? __ldg(p.index + r) : r;
-        s[j] = id >= 0 && id < p.x_rows ? id : p.x_rows;       // outside the matrix: zeros
-      }
+      const int half = ((it.rows + 15) & ~15) >> 1, first = it.row0 + static_cast<int>(rank) * half, wide = half / GC_BOX, boxes = wide + half % GC_BOX / 8;
       const uint32_t bytes = 2 * (GC_A_BYTES + half * GC_K * 2);
+      int4 src;
+      if (GATHER) {
+        int* id = reinterpret_cast<int*>(&src);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // columns past the item's rows are not used: they repeat its last row
+          id[j] = __ldg(p.index + min(first + 4 * lane + j, it.row0 + it.rows - 1));
+          if (id[j] < 0 || id[j] >= p.x_rows) id[j] = p.x_rows;       // outside the matrix: zeros
+        }
+      }
       for (int k = 0; k < p.slices; ++k) {
         if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
-        unsigned char* sa = smem + st * GC_STAGE;
+        unsigned char* sa = smem + st * stage;
         const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
         if (tc::elect_one()) {
           if (rank == 0) tc::mbar_expect_tx(&full[st], bytes);
@@ -169,9 +206,14 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
           }
         }
         __syncwarp();
-        if (4 * lane < half) tma_gather4_pair(sa + GC_A_BYTES + lane * 512, &p.x, k * GC_K, src, bar);
+        if (GATHER) {
+          if (4 * lane < half) tma_gather4_pair(sa + GC_A_BYTES + lane * 512, &p.x, k * GC_K, src, bar);
+        } else if (lane < boxes) {
+          const int r = lane < wide ? GC_BOX * lane : GC_BOX * wide + 8 * (lane - wide);
+          tma_load_2d_pair(sa + GC_A_BYTES + r * GC_K * 2, lane < wide ? &p.x : &p.x8, k * GC_K, first + r, bar);
+        }
         __syncwarp();
-        if (++st == GC_STAGES) { st = 0; ph ^= 1; }
+        if (++st == stages) { st = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1 && rank == 0) {
@@ -180,14 +222,14 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
       const GcItem it = gc_item(tab, item, p.blocks, e);
-      const uint32_t ab = ti & 1u, n = (it.rows + 15) & ~15, idesc = p.bf16 ? tc::idesc_bf16(256, n) : tc::idesc_f16(256, n);
-      if (ti >= 2 && !(ok = tc::mbar_wait(&acc_empty[ab], ((ti >> 1) - 1) & 1))) break;    // read out two items ago
+      const uint32_t ab = ti & 1u, n = (it.rows + 15) & ~15, idesc = BF16 ? tc::idesc_bf16(256, n) : tc::idesc_f16(256, n);
+      if (ti >= 2 && !(ok = tc::mbar_wait_cluster(&acc_empty[ab], ((ti >> 1) - 1) & 1))) break;    // read out two items ago
       tc::fence_after_sync();
       for (int k = 0; k < p.slices; ++k) {
         if (!(ok = tc::mbar_wait(&full[st], ph))) break;
         tc::fence_after_sync();
         if (tc::elect_one()) {
-          const uint32_t sa = tc::smem_u32(smem + st * GC_STAGE);
+          const uint32_t sa = tc::smem_u32(smem + st * stage);
           const uint64_t ad = gc_desc(sa), bd = gc_desc(sa + GC_A_BYTES);
 #pragma unroll
           for (int kk = 0; kk < GC_K / 16; ++kk)
@@ -195,7 +237,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
           tc::mma_commit_pair(&empty[st]);
         }
         __syncwarp();
-        if (++st == GC_STAGES) { st = 0; ph ^= 1; }
+        if (++st == stages) { st = 0; ph ^= 1; }
       }
       if (ok && tc::elect_one()) tc::mma_commit_pair(&acc_full[ab]);
       __syncwarp();
@@ -203,6 +245,8 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   } else if (warp >= GC_EPI0) {
     // ------------------------------------------------------------------ epilogue: lane quarter q, every other block of 32 rows
     const int q = warp & 3, half = (warp - GC_EPI0) >> 2;
+    constexpr int WIDE = GLU ? 16 : 32, PITCH = GLU ? 48 : GC_TURN_PITCH, PIECES = WIDE / 8;      // columns of y a warp has, bytes between rows, 16-byte pieces
+    unsigned char* const mine = turn + (warp - GC_EPI0) * GC_TURN_BYTES;
     uint32_t ti = 0;
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
@@ -211,30 +255,57 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (!(ok = tc::mbar_wait(&acc_full[ab], (ti >> 1) & 1))) break;
       tc::fence_after_sync();
       const uint32_t acc = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + ab * GC_ROWS;
-      const int col = GLU ? it.block * 128 + static_cast<int>(rank) * 64 + 16 * q + (lane & 15) : it.block * 256 + static_cast<int>(rank) * 128 + 32 * q + lane;
+      const int col0 = (it.block * 2 + static_cast<int>(rank)) * (GLU ? 64 : 128) + WIDE * q;
 #pragma unroll 1
       for (int c0 = 32 * half; c0 < it.rows; c0 += 64) {
-        float v[32];
-        tc::tmem_ld32(acc + c0, v);
-        if (GLU) {
-          const int up = lane >> 4;
+        if (F32) {
+          // a lane owns a column: a warp's store is 128 bytes of a row of y
+          float v[32];
+          tc::tmem_ld32(acc + c0, v);
+          float* out = static_cast<float*>(p.y) + static_cast<int64_t>(it.row0 + c0) * p.N + col0 + lane;
+          if (col0 + lane < p.N)
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float other = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
-            const int row = c0 + c + up;
-            if (row < it.rows && col < p.N)
-              store_act(p.y, p.y_dtype, static_cast<int64_t>(it.row0 + row) * p.N + col, up ? silu_mul(other, v[c + 1]) : silu_mul(v[c], other));
-          }
-        } else if (col < p.N) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (c0 + c < it.rows) store_act(p.y, p.y_dtype, static_cast<int64_t>(it.row0 + c0 + c) * p.N + col, v[c]);
+            for (int c = 0; c < 32; ++c)
+              if (c0 + c < it.rows) out[static_cast<int64_t>(c) * p.N] = v[c];
+          continue;
         }
+        uint32_t lo[16], hi[16];
+        tc::tmem_ld_frag32(acc + c0, lo);
+        tc::tmem_ld_frag32(acc + (16u << 16) + c0, hi);
+        tc::tmem_ld_wait(lo, hi);
+        const uint32_t at = tc::smem_u32(mine) + ((lane & 7) + 8 * (lane >> 4)) * PITCH + 16 * ((lane >> 3) & 1);
+        if (GLU) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) lo[i] = __float_as_uint(silu_mul(__uint_as_float(lo[i]), __uint_as_float(hi[i])));
+        }
+#pragma unroll
+        for (int h = 0; h < (GLU ? 1 : 2); ++h) {
+          uint32_t m[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m[i] = gc_pack<BF16>(__uint_as_float(h ? hi[2 * i] : lo[2 * i]), __uint_as_float(h ? hi[2 * i + 1] : lo[2 * i + 1]));
+          stmatrix_x4_trans(at + 32 * h, m[0], m[1], m[2], m[3]);
+          stmatrix_x4_trans(at + 32 * h + 16 * PITCH, m[4], m[5], m[6], m[7]);
+        }
+        __syncwarp();
+        uint16_t* out = static_cast<uint16_t*>(p.y) + static_cast<int64_t>(it.row0 + c0) * p.N + col0;
+        if (p.vec) {
+#pragma unroll
+          for (int u = 0; u < PIECES; ++u) {
+            const int r = (32 / PIECES) * u + lane / PIECES, pc = lane % PIECES;
+            if (c0 + r < it.rows && col0 + 8 * pc < p.N)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * p.N + 8 * pc) = *reinterpret_cast<const uint4*>(mine + r * PITCH + 16 * pc);
+          }
+        } else {
+          const int c = lane % WIDE;
+#pragma unroll 4
+          for (int r = lane / WIDE; r < 32; r += 32 / WIDE)
+            if (c0 + r < it.rows && col0 + c < p.N) out[static_cast<int64_t>(r) * p.N + c] = *reinterpret_cast<const uint16_t*>(mine + r * PITCH + 2 * c);
+        }
+        __syncwarp();
       }
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(tc::cluster_map(tc::smem_u32(&acc_empty[ab]), 0)) : "memory");
+      if (lane == 0) tc::mbar_arrive_release_cluster(tc::cluster_map(tc::smem_u32(&acc_empty[ab]), 0));
     }
   }
   tc::fence_before_sync();
@@ -243,6 +314,12 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   tc::cluster_wait();                          // nothing of the other CTA reaches into this one any more
   if (warp == 2) tc::tmem_dealloc_pair(tmem_base, 512);
 }
+
+static void (*const GC_KERNELS[])(const GcParams) = {
+    grouped_tc_kernel<false, false, false, false>, grouped_tc_kernel<false, false, false, true>, grouped_tc_kernel<false, true, false, false>,
+    grouped_tc_kernel<false, true, false, true>,   grouped_tc_kernel<true, false, false, false>, grouped_tc_kernel<true, false, false, true>,
+    grouped_tc_kernel<true, true, false, false>,   grouped_tc_kernel<true, true, false, true>,   grouped_tc_kernel<false, false, true, false>,
+    grouped_tc_kernel<false, false, true, true>};
 
 int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   const int64_t blocks = (a.N + (a.glu ? 127 : 255)) / (a.glu ? 128 : 256);
@@ -253,8 +330,8 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   const cuuint64_t K = a.K, N = a.N, E = a.E;
   {
     const cuuint64_t dims[2] = {K, static_cast<cuuint64_t>(a.x_rows)}, strides[1] = {K * 2};
-    const cuuint32_t box[2] = {GC_K, 1};
-    if (!encode_map16(&p.x, a.x, 2, dims, strides, box)) return BM_ERR_UNSUPPORTED;
+    const cuuint32_t box[2] = {GC_K, a.index ? 1u : static_cast<cuuint32_t>(GC_BOX)}, box8[2] = {GC_K, 8};
+    if (!encode_map16(&p.x, a.x, 2, dims, strides, box) || (!a.index && !encode_map16(&p.x8, a.x, 2, dims, strides, box8))) return BM_ERR_UNSUPPORTED;
   }
   if (a.glu) {
     const cuuint64_t dims[4] = {K, N, 2, E}, strides[3] = {K * 2, N * K * 2, 2 * N * K * 2};
@@ -268,15 +345,16 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   p.offsets = a.offsets; p.index = a.index; p.y = a.y;
   p.x_rows = a.x_rows; p.rows = a.rows; p.N = a.N; p.E = a.E;
   p.slices = (a.K + GC_K - 1) / GC_K; p.blocks = static_cast<int>(blocks);
-  p.y_dtype = a.y_dtype; p.bf16 = a.dtype == BM_BF16;
+  p.vec = a.N % 8 == 0 && aligned16(a.y);
+  const bool f32 = a.y_dtype == BM_F32;
+  if (f32 && (a.glu || a.index)) return BM_ERR_UNSUPPORTED;
   static PerDeviceOnce once;
   static int grids[MAX_DEVICES];
   int dev = -1;
   BM_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= MAX_DEVICES) return BM_ERR_UNSUPPORTED;
   if (!once.is_done(dev)) {
-    for (auto* kernel : {grouped_tc_kernel<true>, grouped_tc_kernel<false>})
-      BM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gc_smem_bytes(GC_MAX_E)));
+    for (auto& k : GC_KERNELS) BM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, gc_smem_bytes(GC_MAX_E)));
     BM_CUDA(cudaDeviceGetAttribute(&grids[dev], cudaDevAttrMultiProcessorCount, dev));
     grids[dev] &= ~1;
     once.mark(dev);
@@ -284,7 +362,8 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   // items there can be: every group that has rows ends in a piece of its own
   const int64_t most = (static_cast<int64_t>(a.rows) / GC_ROWS + (a.E < a.rows ? a.E : a.rows)) * blocks;
   const int grid = most * 2 < grids[dev] ? static_cast<int>(most) * 2 : grids[dev];
-  BM_CUDA(launch_after(a.after, 2, a.glu ? grouped_tc_kernel<true> : grouped_tc_kernel<false>, dim3(grid), GC_THREADS, gc_smem_bytes(a.E), st, p));
+  const int which = (f32 ? 4 : (a.glu ? 2 : 0) + (a.index ? 1 : 0)) * 2 + (a.dtype == BM_BF16);
+  BM_CUDA(launch_after(a.after, 2, GC_KERNELS[which], dim3(grid), GC_THREADS, gc_smem_bytes(a.E), st, p));
   BM_LAUNCH_CHECK("grouped_tc_kernel");
   return BM_OK;
 }

@@ -334,9 +334,12 @@ PyObject* grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             "grouped_linear: out must be contiguous [rows, N] of x's type and device");
     const c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor y = out.defined() ? out : at::empty({rows, w.size(1)}, x.options());
+    const size_t need = tok.defined() ? bm_grouped_linear_workspace_bytes(static_cast<int32_t>(x.size(1)), static_cast<int32_t>(w.size(0)), static_cast<int32_t>(rows)) : 0;
+    at::Tensor ws;
+    if (need) ws = scratch(need, x);
     check(bm_grouped_linear(x.data_ptr(), dtype, w.data_ptr(), static_cast<int32_t>(x.size(0)), static_cast<int32_t>(x.size(1)),
                             static_cast<int32_t>(w.size(1)), static_cast<int32_t>(w.size(0)), static_cast<const int32_t*>(off.data_ptr()),
-                            static_cast<const int32_t*>(ptr(tok)), static_cast<int32_t>(rows), y.data_ptr(), stream_of(x.device())));
+                            static_cast<const int32_t*>(ptr(tok)), static_cast<int32_t>(rows), y.data_ptr(), ptr(ws), need, stream_of(x.device())));
     return THPVariable_Wrap(y);
   });
 }

@@ -259,9 +259,12 @@ BM_API int bm_dense_mlp_forward(const void* x, int x_dtype, const uint16_t* w_ga
  * y[i] = x[row(i)] . w[e]^T for expert_offsets[e] <= i < expert_offsets[e + 1]: w [E, N, K], y [rows, N], row(i) = token_indices[i]
  * (int32 [rows]; an entry outside [0, x_rows) stands for a row of zeros), or i where token_indices is NULL (then rows <= x_rows).
  * expert_offsets int32 [E + 1] on the device, ascending; entries are limited to [0, rows].  Rows of y that no expert owns, such as
- * those behind expert_offsets[E], are left as they were. */
+ * those behind expert_offsets[E], are left as they were.  A list of many rows an expert is brought into expert order first: with indices the
+ * call needs the workspace of bm_grouped_linear_workspace_bytes (0 for short lists), without them none. */
+BM_API size_t bm_grouped_linear_workspace_bytes(int32_t K, int32_t E, int32_t rows);
 BM_API int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_rows, int32_t K, int32_t N, int32_t E,
-                             const int32_t* expert_offsets, const int32_t* token_indices, int32_t rows, void* y, void* stream);
+                             const int32_t* expert_offsets, const int32_t* token_indices, int32_t rows, void* y, void* workspace,
+                             size_t workspace_bytes, void* stream);
 /* Dense SwiGLU experts of a MoE block for a given selection (_run_super_experts of bitsmoe/models/base_block.py:291-307, without its
  * host round trips):  y[t] = residual[t] + sum over slots s of topk_w[t, s] * w_down[e] . (silu(gate_e . x[t]) * (up_e . x[t])),
  * e = global_to_local[topk_idx[t, s]] (the id itself when the map is NULL, and then num_routed must equal num_local); slots whose id

@@ -293,10 +293,12 @@ def test_c_entry_refusals():
     p = x.data_ptr()
     st = capi.stream_ptr(torch.device(DEV))
     off = torch.zeros(4, dtype=torch.int32, device=DEV).data_ptr()
-    assert lib.bm_grouped_linear(p, 0, p, 8, 0, 4, 1, off, None, 8, p, st) == 1
-    assert lib.bm_grouped_linear(p, 2, p, 8, 64, 4, 1, off, None, 8, p, st) == 1
-    assert lib.bm_grouped_linear(p, 0, None, 8, 64, 4, 1, off, None, 8, p, st) == 1
-    assert lib.bm_grouped_linear(p, 0, p, 4, 64, 4, 1, off, None, 8, p, st) == 1
+    assert lib.bm_grouped_linear(p, 0, p, 8, 0, 4, 1, off, None, 8, p, None, 0, st) == 1
+    assert lib.bm_grouped_linear(p, 2, p, 8, 64, 4, 1, off, None, 8, p, None, 0, st) == 1
+    assert lib.bm_grouped_linear(p, 0, None, 8, 64, 4, 1, off, None, 8, p, None, 0, st) == 1
+    assert lib.bm_grouped_linear(p, 0, p, 4, 64, 4, 1, off, None, 8, p, None, 0, st) == 1
+    assert lib.bm_grouped_linear_workspace_bytes(64, 1, 0) == 0 and lib.bm_grouped_linear_workspace_bytes(64, 2, 5000) >= 5000 * 128
+    assert lib.bm_grouped_linear(p, 0, p, 8, 64, 4, 2, off, off, 5000, p, p, 4999 * 128, st) == 4
     need = lib.bm_dense_experts_workspace_bytes(8, 2, 1, 64, 32)
     assert need > 0 and lib.bm_dense_experts_workspace_bytes(0, 2, 1, 64, 32) == 0
     assert lib.bm_dense_experts_forward(p, 0, off, off, None, 1, 8, 2, 1, p, p, 64, 32, None, p, p, need - 1, st) == 4
