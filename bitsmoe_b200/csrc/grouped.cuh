@@ -5,6 +5,13 @@
 
 namespace bm {
 
+// For every slot of a selection [T, k]: its place among the routed assignments (token_indices, offsets as bm_route_build makes them), or -1.
+struct SlotArgs {
+  const int32_t *topk_idx, *map, *token_indices, *offsets;
+  int32_t* pos;                // [T * k]; null: nothing to do
+  int slots, k, E, num_routed;
+};
+
 // y[i][n] = sum_k x[row(i)][k] * w[e][n][k] for offsets[e] <= i < offsets[e + 1], row(i) = index[i] (i itself when null).
 // glu: w holds 2 N rows per expert, gate rows before up rows, and y[i][n] = silu(row n) * row (N + n).
 // offsets null: one group of all `rows` rows.
@@ -19,8 +26,30 @@ struct GroupedArgs {
   int glu;
   int expected;                // rows that the groups are expected to have, 0 = `rows`
   void* gathered;              // with an index: room for [rows, K], 16-byte aligned, or null
+  SlotArgs slots;              // worked out beside the products
   LaunchAfter after;
 };
+
+__device__ __forceinline__ int slot_expert(const SlotArgs& a, int i) {
+  const int id = a.topk_idx[i];
+  if (id < 0 || id >= a.num_routed) return -1;
+  const int e = a.map ? a.map[id] : id;
+  return e >= 0 && e < a.E ? e : -1;
+}
+// Slot i's place: the routing build keeps an expert's list in ascending (token, slot) order, so the token is found by bisection; an expert
+// may be named twice.
+__device__ __forceinline__ int slot_place(const SlotArgs& a, int i) {
+  const int e = slot_expert(a, i), t = i / a.k;
+  if (e < 0) return -1;
+  int lo = a.offsets[e], hi = a.offsets[e + 1];
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.token_indices[mid] < t) lo = mid + 1;
+    else hi = mid;
+  }
+  for (int j = t * a.k; j < i; ++j) lo += slot_expert(a, j) == e;
+  return lo;
+}
 
 // The rows of group e, whatever the caller's table holds: inside [0, rows), ends not before they start.
 __device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int rows) {

@@ -24,19 +24,22 @@ namespace bm {
 
 bool encode_map16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 
-constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_MAX_STAGES = 12, GC_MAX_E = 1024;
+constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_MAX_STAGES = 24, GC_MAX_E = 1024;
 constexpr int GC_TURN_PITCH = 80, GC_TURN_BYTES = 32 * GC_TURN_PITCH;      // 32 rows of 64 (gated pair: 32) bytes: eight rows hit eight bank groups
 constexpr int GC_A_BYTES = 128 * GC_K * 2, GC_BOX = 32;
-// The ring: stages of 128 weight rows and half of the rows of the longest item that the offsets make, 6 of 32 KB to 11 of 17 KB.
+// The ring: stages of 128 weight rows and half of the rows of the longest item that the offsets make, 6 of 32 KB to 24 of 5 KB.
 constexpr int GC_RING = 6 * 2 * GC_A_BYTES;
+// Where the items would leave most pairs idle they are cut along the weight rows: a CTA takes 32 `quarters` of them instead of 128, the rest of
+// its rows of the accumulator is not looked at.
 constexpr int gc_smem_bytes(int E) { return GC_RING + GC_EPI_WARPS * GC_TURN_BYTES + 1024 + (3 * E + 1) * 4; }
 
 struct GcParams {
-  CUtensorMap x, x8, w;        // x: 32 rows in order (one row of a gather), or 8
+  CUtensorMap x, x8, w, w32;   // x: 32 rows in order (one row of a gather), or 8; w: 128 weight rows, or 32 (gated pair: 16 and 16)
   const int32_t* offsets;
   const int32_t* index;
   void* y;
-  int x_rows, rows, N, E, slices, blocks, vec;     // blocks: items along the weight rows; vec: y takes 16-byte stores
+  int x_rows, rows, N, E, slices, vec;     // vec: y takes 16-byte stores
+  SlotArgs slots;
 };
 
 // Copies into this CTA's shared memory, signalled on `bar` (shared::cluster address, of either CTA of the pair): four rows, tiles.
@@ -70,9 +73,10 @@ __device__ __forceinline__ uint64_t gc_desc(uint32_t saddr) {
   return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// The items of the groups: group e has ceil(rows / 256) pieces of (nearly) equal size, each with `blocks` items.
+// Group e has ceil(rows / 256) pieces of (nearly) equal size, each with `blocks` items along the weight rows.
 struct GcTable {
-  const int *first, *start, *count;     // [E + 1] items before the group; its first row; its rows
+  const int *first, *start, *count;     // [E + 1] pieces before the group; its first row; its rows
+  int blocks;
 };
 // Rows of the pieces of a group of n rows, a multiple of 16 (a lesser last one apart).
 __device__ __forceinline__ int gc_piece(int n) {
@@ -82,14 +86,15 @@ __device__ __forceinline__ int gc_piece(int n) {
 struct GcItem {
   int e, row0, rows, block;
 };
-__device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int blocks, int& e) {
-  while (item >= tab.first[e + 1]) ++e;
-  const int local = item - tab.first[e], piece = local / blocks, n = tab.count[e], size = gc_piece(n);
+__device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int& e) {
+  const int piece = item / tab.blocks;
+  while (piece >= tab.first[e + 1]) ++e;
+  const int i = piece - tab.first[e], n = tab.count[e], size = gc_piece(n);
   GcItem it;
   it.e = e;
-  it.block = local - piece * blocks;
-  it.row0 = tab.start[e] + piece * size;
-  it.rows = min(size, n - piece * size);       // at least one: size < 256 only where 16 (pieces - 1) < n / pieces
+  it.block = item - piece * tab.blocks;
+  it.row0 = tab.start[e] + i * size;
+  it.rows = min(size, n - i * size);       // at least one: size < 256 only where 16 (pieces - 1) < n / pieces
   return it;
 }
 
@@ -131,10 +136,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     }
     tc::mbar_init_fence();
   }
+  if (threadIdx.x == 32) {
+    for (const CUtensorMap* m : {&p.x, &p.x8, &p.w, &p.w32}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+  }
   __syncthreads();
   tc::cluster_arrive();
-  tc::cluster_wait();                          // both CTAs run and their barriers are set up
-  if (warp == 2) tc::tmem_alloc_pair(&tmem_slot, 512);
   grid_launch_dependents();
   grid_wait();
   for (int e = threadIdx.x; e < p.E; e += GC_THREADS) {
@@ -142,6 +148,8 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     t_start[e] = r.x;
     t_count[e] = r.y - r.x;
   }
+  tc::cluster_wait();                          // both CTAs run and their barriers are set up
+  if (warp == 2) tc::tmem_alloc_pair(&tmem_slot, 512);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -151,7 +159,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int e = e0 + lane, n = e < p.E ? t_count[e] : 0;
       most = max(most, gc_piece(n));
-      int incl = (n + GC_ROWS - 1) / GC_ROWS * p.blocks;
+      int incl = (n + GC_ROWS - 1) / GC_ROWS;
       const int mine = incl;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -168,9 +176,12 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     }
   }
   __syncthreads();
-  const GcTable tab{t_first, t_start, t_count};
-  const int items = t_first[p.E], pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int stage = GC_A_BYTES + longest / 2 * GC_K * 2, stages = min(GC_RING / stage, GC_MAX_STAGES);
+  const int pieces = t_first[p.E], pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  constexpr int QUARTER = GLU ? 32 : 64;       // columns of y of a pair's quarter
+  const int cols1 = (p.N + QUARTER - 1) / QUARTER, quarters = static_cast<int64_t>(pieces) * cols1 <= pairs ? 1 : static_cast<int64_t>(pieces) * ((cols1 + 1) / 2) <= pairs ? 2 : 4;
+  const GcTable tab{t_first, t_start, t_count, (cols1 + quarters - 1) / quarters};
+  const int items = pieces * tab.blocks, a_bytes = quarters * (GC_A_BYTES / 4);
+  const int stage = a_bytes + longest / 2 * GC_K * 2, stages = min(GC_RING / stage, GC_MAX_STAGES);
   bool ok = true;
 
   if (warp == 0) {
@@ -178,9 +189,9 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     uint32_t st = 0, ph = 0;
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs) {
-      const GcItem it = gc_item(tab, item, p.blocks, e);
+      const GcItem it = gc_item(tab, item, e);
       const int half = ((it.rows + 15) & ~15) >> 1, first = it.row0 + static_cast<int>(rank) * half, wide = half / GC_BOX, boxes = wide + half % GC_BOX / 8;
-      const uint32_t bytes = 2 * (GC_A_BYTES + half * GC_K * 2);
+      const uint32_t bytes = 2 * (a_bytes + half * GC_K * 2);
       int4 src;
       if (GATHER) {
         int* id = reinterpret_cast<int*>(&src);
@@ -197,20 +208,21 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
         if (tc::elect_one()) {
           if (rank == 0) tc::mbar_expect_tx(&full[st], bytes);
+          const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
           if (GLU) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w, k * GC_K, it.block * 128 + static_cast<int>(rank) * 64 + 16 * b, 0, it.e, bar);
+            for (int b = 0; b < quarters; ++b) tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k * GC_K, col0 + 16 * b, 0, it.e, bar);
+          } else if (quarters == 4) {
+            tma_load_3d_pair(sa, &p.w, k * GC_K, col0, it.e, bar);
           } else {
-            tma_load_3d_pair(sa, &p.w, k * GC_K, it.block * 256 + static_cast<int>(rank) * 128, it.e, bar);
+            for (int b = 0; b < quarters; ++b) tma_load_3d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k * GC_K, col0 + 32 * b, it.e, bar);
           }
         }
         __syncwarp();
         if (GATHER) {
-          if (4 * lane < half) tma_gather4_pair(sa + GC_A_BYTES + lane * 512, &p.x, k * GC_K, src, bar);
+          if (4 * lane < half) tma_gather4_pair(sa + a_bytes + lane * 512, &p.x, k * GC_K, src, bar);
         } else if (lane < boxes) {
           const int r = lane < wide ? GC_BOX * lane : GC_BOX * wide + 8 * (lane - wide);
-          tma_load_2d_pair(sa + GC_A_BYTES + r * GC_K * 2, lane < wide ? &p.x : &p.x8, k * GC_K, first + r, bar);
+          tma_load_2d_pair(sa + a_bytes + r * GC_K * 2, lane < wide ? &p.x : &p.x8, k * GC_K, first + r, bar);
         }
         __syncwarp();
         if (++st == stages) { st = 0; ph ^= 1; }
@@ -221,7 +233,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     uint32_t st = 0, ph = 0, ti = 0;
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
-      const GcItem it = gc_item(tab, item, p.blocks, e);
+      const GcItem it = gc_item(tab, item, e);
       const uint32_t ab = ti & 1u, n = (it.rows + 15) & ~15, idesc = BF16 ? tc::idesc_bf16(256, n) : tc::idesc_f16(256, n);
       if (ti >= 2 && !(ok = tc::mbar_wait_cluster(&acc_empty[ab], ((ti >> 1) - 1) & 1))) break;    // read out two items ago
       tc::fence_after_sync();
@@ -230,7 +242,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         tc::fence_after_sync();
         if (tc::elect_one()) {
           const uint32_t sa = tc::smem_u32(smem + st * stage);
-          const uint64_t ad = gc_desc(sa), bd = gc_desc(sa + GC_A_BYTES);
+          const uint64_t ad = gc_desc(sa), bd = gc_desc(sa + a_bytes);
 #pragma unroll
           for (int kk = 0; kk < GC_K / 16; ++kk)
             tc::mma_f16_pair(tmem_base + ab * GC_ROWS, ad + 2 * kk, bd + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
@@ -242,6 +254,10 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (ok && tc::elect_one()) tc::mma_commit_pair(&acc_full[ab]);
       __syncwarp();
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ places of the slots, for whoever sums over a token's experts
+    if (p.slots.pos)
+      for (int i = blockIdx.x * 32 + lane; i < p.slots.slots; i += gridDim.x * 32) p.slots.pos[i] = slot_place(p.slots, i);
   } else if (warp >= GC_EPI0) {
     // ------------------------------------------------------------------ epilogue: lane quarter q, every other block of 32 rows
     const int q = warp & 3, half = (warp - GC_EPI0) >> 2;
@@ -250,14 +266,14 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     uint32_t ti = 0;
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
-      const GcItem it = gc_item(tab, item, p.blocks, e);
+      const GcItem it = gc_item(tab, item, e);
       const uint32_t ab = ti & 1u;
       if (!(ok = tc::mbar_wait(&acc_full[ab], (ti >> 1) & 1))) break;
       tc::fence_after_sync();
       const uint32_t acc = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + ab * GC_ROWS;
-      const int col0 = (it.block * 2 + static_cast<int>(rank)) * (GLU ? 64 : 128) + WIDE * q;
+      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2) + WIDE * q;
 #pragma unroll 1
-      for (int c0 = 32 * half; c0 < it.rows; c0 += 64) {
+      for (int c0 = q < quarters ? 32 * half : it.rows; c0 < it.rows; c0 += 64) {
         if (F32) {
           // a lane owns a column: a warp's store is 128 bytes of a row of y
           float v[32];
@@ -322,9 +338,10 @@ static void (*const GC_KERNELS[])(const GcParams) = {
     grouped_tc_kernel<false, false, true, true>};
 
 int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
-  const int64_t blocks = (a.N + (a.glu ? 127 : 255)) / (a.glu ? 128 : 256);
-  if (a.K % 8 != 0 || a.x_rows == 0 || a.E > GC_MAX_E || !aligned16(a.x, a.w) || (static_cast<int64_t>(a.rows) / GC_ROWS + a.E + 1) * blocks > 0x7fffffff)
-    return BM_ERR_UNSUPPORTED;
+  const int64_t quarters = (a.N + (a.glu ? 31 : 63)) / (a.glu ? 32 : 64);
+  // pieces there can be: every group that has rows ends in one of its own
+  const int64_t most = (static_cast<int64_t>(a.rows) / GC_ROWS + (a.E < a.rows ? a.E : a.rows)) * quarters;
+  if (a.K % 8 != 0 || a.x_rows == 0 || a.E > GC_MAX_E || !aligned16(a.x, a.w) || most > 0x3fffffff) return BM_ERR_UNSUPPORTED;
   GcParams p;
   memset(&p, 0, sizeof(p));
   const cuuint64_t K = a.K, N = a.N, E = a.E;
@@ -336,16 +353,17 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   if (a.glu) {
     const cuuint64_t dims[4] = {K, N, 2, E}, strides[3] = {K * 2, N * K * 2, 2 * N * K * 2};
     const cuuint32_t box[4] = {GC_K, 16, 2, 1};
-    if (!encode_map16(&p.w, a.w, 4, dims, strides, box)) return BM_ERR_UNSUPPORTED;
+    if (!encode_map16(&p.w32, a.w, 4, dims, strides, box)) return BM_ERR_UNSUPPORTED;
   } else {
     const cuuint64_t dims[3] = {K, N, E}, strides[2] = {K * 2, N * K * 2};
-    const cuuint32_t box[3] = {GC_K, 128, 1};
-    if (!encode_map16(&p.w, a.w, 3, dims, strides, box)) return BM_ERR_UNSUPPORTED;
+    const cuuint32_t box[3] = {GC_K, 128, 1}, box32[3] = {GC_K, 32, 1};
+    if (!encode_map16(&p.w, a.w, 3, dims, strides, box) || !encode_map16(&p.w32, a.w, 3, dims, strides, box32)) return BM_ERR_UNSUPPORTED;
   }
   p.offsets = a.offsets; p.index = a.index; p.y = a.y;
   p.x_rows = a.x_rows; p.rows = a.rows; p.N = a.N; p.E = a.E;
-  p.slices = (a.K + GC_K - 1) / GC_K; p.blocks = static_cast<int>(blocks);
+  p.slices = (a.K + GC_K - 1) / GC_K;
   p.vec = a.N % 8 == 0 && aligned16(a.y);
+  p.slots = a.slots;
   const bool f32 = a.y_dtype == BM_F32;
   if (f32 && (a.glu || a.index)) return BM_ERR_UNSUPPORTED;
   static PerDeviceOnce once;
@@ -359,8 +377,6 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
     grids[dev] &= ~1;
     once.mark(dev);
   }
-  // items there can be: every group that has rows ends in a piece of its own
-  const int64_t most = (static_cast<int64_t>(a.rows) / GC_ROWS + (a.E < a.rows ? a.E : a.rows)) * blocks;
   const int grid = most * 2 < grids[dev] ? static_cast<int>(most) * 2 : grids[dev];
   const int which = (f32 ? 4 : (a.glu ? 2 : 0) + (a.index ? 1 : 0)) * 2 + (a.dtype == BM_BF16);
   BM_CUDA(launch_after(a.after, 2, GC_KERNELS[which], dim3(grid), GC_THREADS, gc_smem_bytes(a.E), st, p));
