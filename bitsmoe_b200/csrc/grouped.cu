@@ -19,9 +19,9 @@ __device__ __forceinline__ float load16(const void* p, int64_t i) {
 }
 
 // Rows a group from which a pass over the rows of x costs less than fetching them four at a time for every item.  128 groups, K 2048, N 1536, us
-// by a pass first / by gather copies / with the rows in order: 8 rows 148 / 139 / 141, 32 rows 155 / 142 / 146, 48 rows 162 / 152 / 151, 64 rows 162 / 176 /
-// 150, 128 rows 179 / 275 / 157, 512 rows 401 / 894 / 350: four rows of 128 bytes take the copy engine 57 cycles.
-constexpr int GATHER_ROWS = 48;
+// by a pass first / by gather copies / with the rows in order: 8 rows 148 / 128 / 124, 32 rows 155 / 135 / 130, 48 rows 155 / 146 / 134, 64 rows 166 / 198 /
+// 142, 128 rows 180 / 290 / 155, 512 rows 400 / 900 / 340: four rows of 128 bytes take the copy engine 57 cycles.
+constexpr int GATHER_ROWS = 56;
 
 // Any shape and alignment: a CTA takes 16 rows of a group and 64 output columns, element loads, fp32 FMA.
 template <int D, bool GLU>
@@ -278,6 +278,7 @@ extern "C" int bm_grouped_linear(const void* x, int dtype, const void* w, int32_
   a.gathered = need ? workspace : nullptr;
   a.x = x; a.w = w; a.offsets = expert_offsets; a.index = token_indices; a.y = y;
   a.x_rows = x_rows; a.rows = rows; a.K = K; a.N = N; a.E = E; a.dtype = a.y_dtype = dtype;
+  a.after = AFTER_READS;
   return launch_grouped(a, static_cast<cudaStream_t>(stream));
 }
 

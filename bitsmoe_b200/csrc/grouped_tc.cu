@@ -5,7 +5,7 @@
 // (expert, up to 256 of its rows, 256 weight rows): each CTA loads 128 weight rows and half of the item's rows, and the tensor cores
 // read both halves, so that an SM fetches 32 KB per 64 columns of K for 128 x 256 sums (a lone CTA would need 48, which is more than an SM gets
 // from L2 while its tensor core multiplies them).
-//   warp 0      producer: weight rows and rows of x as tiled copies, or rows of x by tile::gather4 (a lane names four of them), all onto
+//   warp 0      producer: weight rows and rows of x as tiled copies, or rows of x by tile::gather4 (four an instruction), all onto
 //               the even CTA's barrier
 //   warp 1      MMA issue, in the even CTA for both: four tcgen05.mma (M = 256, N = the item's rows, K = 16) per stage
 //   warps 4-11  epilogue: tensor memory -> registers (fragments of 16 weight rows x 8 rows) -> y.  stmatrix turns them round in
@@ -24,10 +24,10 @@ namespace bm {
 
 bool encode_map16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 
-constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_MAX_STAGES = 24, GC_MAX_E = 1024;
+constexpr int GC_THREADS = 384, GC_EPI0 = 4, GC_EPI_WARPS = 8, GC_K = 64, GC_ROWS = 256, GC_MAX_STAGES = 16, GC_MAX_E = 1024;
 constexpr int GC_TURN_PITCH = 80, GC_TURN_BYTES = 32 * GC_TURN_PITCH;      // 32 rows of 64 (gated pair: 32) bytes: eight rows hit eight bank groups
 constexpr int GC_A_BYTES = 128 * GC_K * 2, GC_BOX = 32;
-// The ring: stages of 128 weight rows and half of the rows of the longest item that the offsets make, 6 of 32 KB to 24 of 5 KB.
+// The ring: slices of 128 weight rows and half of the rows of the longest item that the offsets make, a stage holds one, two or four.
 constexpr int GC_RING = 6 * 2 * GC_A_BYTES;
 // Where the items would leave most pairs idle they are cut along the weight rows: a CTA takes 32 `quarters` of them instead of 128, the rest of
 // its rows of the accumulator is not looked at.
@@ -85,6 +85,10 @@ __device__ __forceinline__ int gc_piece(int n) {
 }
 struct GcItem {
   int e, row0, rows, block;
+  __device__ int n() const { return (rows + 15) & ~15; }
+  // A product waits for the sum that the one before wrote: 112 cycles however few rows there are, where 256 rows take 128.  Few rows
+  // get two or four sums that take the products in turn and are added up at the end.
+  __device__ int parts() const { return rows <= 64 ? 4 : rows <= 128 ? 2 : 1; }
 };
 __device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int& e) {
   const int piece = item / tab.blocks;
@@ -119,6 +123,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   __shared__ __align__(8) uint64_t full[GC_MAX_STAGES], empty[GC_MAX_STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int longest;
+  __shared__ int4 rows4[32];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gc_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* const turn = smem + GC_RING;
   int* const t_first = reinterpret_cast<int*>(turn + GC_EPI_WARPS * GC_TURN_BYTES);
@@ -181,7 +186,9 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   const int cols1 = (p.N + QUARTER - 1) / QUARTER, quarters = static_cast<int64_t>(pieces) * cols1 <= pairs ? 1 : static_cast<int64_t>(pieces) * ((cols1 + 1) / 2) <= pairs ? 2 : 4;
   const GcTable tab{t_first, t_start, t_count, (cols1 + quarters - 1) / quarters};
   const int items = pieces * tab.blocks, a_bytes = quarters * (GC_A_BYTES / 4);
-  const int stage = a_bytes + longest / 2 * GC_K * 2, stages = min(GC_RING / stage, GC_MAX_STAGES);
+  // a stage's barriers, waits and commit cost 0.2 us: small slices share them
+  const int slice = a_bytes + longest / 2 * GC_K * 2, sub = slice <= GC_RING / 32 ? 4 : slice <= GC_RING / 10 ? 2 : 1;
+  const int stages = min(GC_RING / (slice * sub), GC_MAX_STAGES);
   bool ok = true;
 
   if (warp == 0) {
@@ -190,39 +197,48 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs) {
       const GcItem it = gc_item(tab, item, e);
-      const int half = ((it.rows + 15) & ~15) >> 1, first = it.row0 + static_cast<int>(rank) * half, wide = half / GC_BOX, boxes = wide + half % GC_BOX / 8;
-      const uint32_t bytes = 2 * (a_bytes + half * GC_K * 2);
-      int4 src;
+      const int half = it.n() >> 1, first = it.row0 + static_cast<int>(rank) * half;
+      const uint32_t bytes = 2 * (a_bytes + half * GC_K * 2);      // of both CTAs' slices
       if (GATHER) {
-        int* id = reinterpret_cast<int*>(&src);
+        int id[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           // columns past the item's rows are not used: they repeat its last row
           id[j] = __ldg(p.index + min(first + 4 * lane + j, it.row0 + it.rows - 1));
           if (id[j] < 0 || id[j] >= p.x_rows) id[j] = p.x_rows;       // outside the matrix: zeros
         }
+        __syncwarp();
+        rows4[lane] = make_int4(id[0], id[1], id[2], id[3]);
+        __syncwarp();
       }
-      for (int k = 0; k < p.slices; ++k) {
+      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
+      for (int k0 = 0; k0 < p.slices; k0 += sub) {
         if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
-        unsigned char* sa = smem + st * stage;
+        const int cnt = min(sub, p.slices - k0);
+        unsigned char* const s0 = smem + st * (sub * slice);
         const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
         if (tc::elect_one()) {
-          if (rank == 0) tc::mbar_expect_tx(&full[st], bytes);
-          const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
-          if (GLU) {
-            for (int b = 0; b < quarters; ++b) tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k * GC_K, col0 + 16 * b, 0, it.e, bar);
-          } else if (quarters == 4) {
-            tma_load_3d_pair(sa, &p.w, k * GC_K, col0, it.e, bar);
-          } else {
-            for (int b = 0; b < quarters; ++b) tma_load_3d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k * GC_K, col0 + 32 * b, it.e, bar);
+          if (rank == 0) tc::mbar_expect_tx(&full[st], cnt * bytes);
+          for (int j = 0; j < cnt; ++j) {
+            unsigned char* sa = s0 + j * slice;
+            const int k = (k0 + j) * GC_K;
+            if (GLU) {
+              for (int b = 0; b < quarters; ++b) tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 16 * b, 0, it.e, bar);
+            } else if (quarters == 4) {
+              tma_load_3d_pair(sa, &p.w, k, col0, it.e, bar);
+            } else {
+              for (int b = 0; b < quarters; ++b) tma_load_3d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 32 * b, it.e, bar);
+            }
+            unsigned char* const sb = sa + a_bytes;
+            if (GATHER) {
+#pragma unroll 4
+              for (int r = 0; r < half; r += 4) tma_gather4_pair(sb + r * (GC_K * 2), &p.x, k, rows4[r / 4], bar);
+            } else {
+              int r = 0;
+              for (; r + GC_BOX <= half; r += GC_BOX) tma_load_2d_pair(sb + r * (GC_K * 2), &p.x, k, first + r, bar);
+              for (; r < half; r += 8) tma_load_2d_pair(sb + r * (GC_K * 2), &p.x8, k, first + r, bar);
+            }
           }
-        }
-        __syncwarp();
-        if (GATHER) {
-          if (4 * lane < half) tma_gather4_pair(sa + a_bytes + lane * 512, &p.x, k * GC_K, src, bar);
-        } else if (lane < boxes) {
-          const int r = lane < wide ? GC_BOX * lane : GC_BOX * wide + 8 * (lane - wide);
-          tma_load_2d_pair(sa + a_bytes + r * GC_K * 2, lane < wide ? &p.x : &p.x8, k * GC_K, first + r, bar);
         }
         __syncwarp();
         if (++st == stages) { st = 0; ph ^= 1; }
@@ -234,18 +250,21 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
       const GcItem it = gc_item(tab, item, e);
-      const uint32_t ab = ti & 1u, n = (it.rows + 15) & ~15, idesc = BF16 ? tc::idesc_bf16(256, n) : tc::idesc_f16(256, n);
+      const uint32_t ab = ti & 1u, idesc = BF16 ? tc::idesc_bf16(256, it.n()) : tc::idesc_f16(256, it.n()), parts = it.parts(), apart = GC_ROWS / parts;
       if (ti >= 2 && !(ok = tc::mbar_wait_cluster(&acc_empty[ab], ((ti >> 1) - 1) & 1))) break;    // read out two items ago
       tc::fence_after_sync();
-      for (int k = 0; k < p.slices; ++k) {
+      for (int k0 = 0; k0 < p.slices; k0 += sub) {
         if (!(ok = tc::mbar_wait(&full[st], ph))) break;
         tc::fence_after_sync();
         if (tc::elect_one()) {
-          const uint32_t sa = tc::smem_u32(smem + st * stage);
-          const uint64_t ad = gc_desc(sa), bd = gc_desc(sa + a_bytes);
+          const int cnt = min(sub, p.slices - k0);
+          for (int j = 0; j < cnt; ++j) {
+            const uint32_t sa = tc::smem_u32(smem + (st * sub + j) * slice);
+            const uint64_t ad = gc_desc(sa), bd = gc_desc(sa + a_bytes);
 #pragma unroll
-          for (int kk = 0; kk < GC_K / 16; ++kk)
-            tc::mma_f16_pair(tmem_base + ab * GC_ROWS, ad + 2 * kk, bd + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < GC_K / 16; ++kk)
+              tc::mma_f16_pair(tmem_base + ab * GC_ROWS + (kk & (parts - 1)) * apart, ad + 2 * kk, bd + 2 * kk, idesc, k0 + j > 0 || kk >= parts ? 1u : 0u);
+          }
           tc::mma_commit_pair(&empty[st]);
         }
         __syncwarp();
@@ -271,13 +290,19 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (!(ok = tc::mbar_wait(&acc_full[ab], (ti >> 1) & 1))) break;
       tc::fence_after_sync();
       const uint32_t acc = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + ab * GC_ROWS;
-      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2) + WIDE * q;
+      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2) + WIDE * q, parts = it.parts();
 #pragma unroll 1
       for (int c0 = q < quarters ? 32 * half : it.rows; c0 < it.rows; c0 += 64) {
         if (F32) {
           // a lane owns a column: a warp's store is 128 bytes of a row of y
           float v[32];
           tc::tmem_ld32(acc + c0, v);
+          for (int i = 1; i < parts; ++i) {
+            float w[32];
+            tc::tmem_ld32(acc + c0 + i * (GC_ROWS / parts), w);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] += w[c];
+          }
           float* out = static_cast<float*>(p.y) + static_cast<int64_t>(it.row0 + c0) * p.N + col0 + lane;
           if (col0 + lane < p.N)
 #pragma unroll
@@ -289,6 +314,17 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         tc::tmem_ld_frag32(acc + c0, lo);
         tc::tmem_ld_frag32(acc + (16u << 16) + c0, hi);
         tc::tmem_ld_wait(lo, hi);
+        for (int i = 1; i < parts; ++i) {
+          uint32_t l2[16], h2[16];
+          tc::tmem_ld_frag32(acc + c0 + i * (GC_ROWS / parts), l2);
+          tc::tmem_ld_frag32(acc + (16u << 16) + c0 + i * (GC_ROWS / parts), h2);
+          tc::tmem_ld_wait(l2, h2);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            lo[j] = __float_as_uint(__uint_as_float(lo[j]) + __uint_as_float(l2[j]));
+            hi[j] = __float_as_uint(__uint_as_float(hi[j]) + __uint_as_float(h2[j]));
+          }
+        }
         const uint32_t at = tc::smem_u32(mine) + ((lane & 7) + 8 * (lane >> 4)) * PITCH + 16 * ((lane >> 3) & 1);
         if (GLU) {
 #pragma unroll

@@ -339,7 +339,7 @@ extern "C" int bm_linear4(const void* x, int dtype, const uint32_t* payload, con
   a.p[0] = payload; a.s[0] = reinterpret_cast<const __half*>(scale);
   a.x = x; a.residual = residual; a.y = y;
   a.T = T; a.K = K; a.N = N; a.ldx = K; a.ldy = N; a.y_dtype = dtype;
-  return linear4(a, dtype, group, AFTER_ALL, static_cast<cudaStream_t>(stream));
+  return linear4(a, dtype, group, AFTER_READS, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t bm_dense_mlp4_workspace_bytes(int32_t T, int32_t intermediate) {
@@ -365,12 +365,12 @@ extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* g
   const int ldz = static_cast<int>(align_up(intermediate, 8));
   void* z = workspace;
   float* gate = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align_up(static_cast<size_t>(T) * ldz * 2, 256));
-  if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_ALL, st))) return rc;
+  if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_READS, st))) return rc;
   Linear4Args a{};
   a.p[0] = gate_payload; a.p[1] = up_payload;
   a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
   a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.y_dtype = dtype; a.glu = 1;
-  if ((rc = linear4(a, dtype, group, token_gate_w ? AFTER_READS : AFTER_ALL, st))) return rc;
+  if ((rc = linear4(a, dtype, group, AFTER_READS, st))) return rc;
   Linear4Args d{};
   d.p[0] = down_payload; d.s[0] = reinterpret_cast<const __half*>(down_scale);
   d.x = z; d.residual = residual; d.row_gate = token_gate_w ? gate : nullptr; d.y = y;
