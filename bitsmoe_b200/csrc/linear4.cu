@@ -12,7 +12,7 @@
 
 #include <algorithm>
 
-#include "grouped.cuh"
+#include "linear4.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -20,53 +20,21 @@ namespace bm {
 
 int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st);
 
-constexpr int L4_THREADS = 256, L4_WARPS = 8, L4_CHUNK = 128, L4_BATCH = 4;
+constexpr int L4_THREADS = 256, L4_WARPS = 8, L4_CHUNK = 128;
+__host__ __device__ constexpr int l4_batch(int nt) { return nt <= 8 ? 2 : 4; }      // chunks in flight a warp and buffer
+__host__ __device__ constexpr int l4_ctas(int nt) { return nt <= 8 ? 3 : 2; }       // CTAs an SM
 constexpr size_t L4_SMEM = 110 * 1024;          // two CTAs an SM
 
-struct Linear4Args {
-  const uint32_t* p[2];        // codes [N, words]; GLU: gate and up
-  const __half* s[2];          // scales [N, groups]
-  const void* x;               // [T, ldx]
-  const void* residual;        // [T, N] of y's type, or null
-  const float* row_gate;       // factor per token, or null
-  void* y;                     // [T, ldy]
-  int T, K, N, ldx, ldy, words, groups;
-  int glu, y_dtype, vec_x, kwarps, splits, row_blocks;
-};
-
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Eight codes -> four pairs (code i, code i + 4), i = 0 .. 3, as exact numbers -8 .. 7 of the type.
 template <int XD>
-__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&q)[4]) {
-  if (XD == BM_F16) {
-    // 1024 + u and 1024 + 16 u are fp16 numbers with u in their low mantissa bits
-    const __half2 off = __float2half2_rn(1032.f), sixteenth = __float2half2_rn(0.0625f), minus72 = __float2half2_rn(-72.f);
-#pragma unroll
-    for (int h = 0; h < 2; ++h, w >>= 8) {
-      const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x64006400u;
-      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off), b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, minus72);
-      q[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
-      q[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-  } else {
-    const __nv_bfloat162 off = __float2bfloat162_rn(136.f);       // 128 + u
-#pragma unroll
-    for (int i = 0; i < 4; ++i, w >>= 4) {
-      const uint32_t v = (w & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-      q[i] = *reinterpret_cast<const uint32_t*>(&a);
-    }
-  }
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  if (XD == BM_F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // Place of word kw (eight columns of x) among the words of a CTA: the words that a quad's lanes use together are neighbours.
@@ -81,8 +49,8 @@ __device__ __forceinline__ int l4_piece(int place, int n) {
 }
 
 template <int NT, int XD, int WPL>
-__global__ void __launch_bounds__(L4_THREADS, 2) linear4_kernel(const __grid_constant__ Linear4Args a) {
-  constexpr int NB = NT < 8 ? 1 : NT / 8, GPC = 4 / WPL, SPR = (L4_BATCH * GPC + 3) / 4;     // groups a chunk, scale loads per row and batch
+__global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const __grid_constant__ Linear4Args a) {
+  constexpr int NB = NT < 8 ? 1 : NT / 8, GPC = 4 / WPL, L4_BATCH = l4_batch(NT), SPR = (L4_BATCH * GPC + 3) / 4;     // groups a chunk, scale loads per row and batch
   extern __shared__ __align__(16) unsigned char l4_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % a.splits, kw = warp % a.kwarps, rw = warp / a.kwarps, rws = L4_WARPS / a.kwarps;
@@ -90,126 +58,139 @@ __global__ void __launch_bounds__(L4_THREADS, 2) linear4_kernel(const __grid_con
   const int c_first = chunks * split / a.splits, c_end = chunks * (split + 1) / a.splits;           // this CTA's chunks of 128 columns
   const int n0 = blockIdx.y * NT, nn = min(NT, a.T - n0);
   float* const recv = reinterpret_cast<float*>(l4_smem + static_cast<size_t>((chunks + a.splits - 1) / a.splits) * (L4_CHUNK / 8) * NT * 16);
+  const int wc = c_end - c_first, w_first = wc * kw / a.kwarps, w_end = wc * (kw + 1) / a.kwarps;      // this warp's chunks, CTA-relative
+  const int per = a.glu ? 8 : 16, cluster_id = blockIdx.x / a.splits, clusters = gridDim.x / a.splits;
+  // ---- the weights travel a batch ahead of the products, across the ends of units too: where the next batch starts
+  int f_rb = cluster_id, f_c = w_first;
+  const uint32_t *pa, *pc;
+  const __half *sa, *sc;
+  auto rows_of = [&](int rb) {
+    const int r0 = (rb * rws + rw) * per, ra = min(r0 + g, a.N - 1), rc = a.glu ? ra : min(r0 + 8 + g, a.N - 1);
+    pa = a.p[0] + static_cast<int64_t>(ra) * a.words;
+    pc = (a.glu ? a.p[1] : a.p[0]) + static_cast<int64_t>(rc) * a.words;
+    sa = a.s[0] + static_cast<int64_t>(ra) * a.groups;
+    sc = (a.glu ? a.s[1] : a.s[0]) + static_cast<int64_t>(rc) * a.groups;
+  };
+  rows_of(f_rb);
+  auto fetch = [&](uint32_t (&wd)[2][L4_BATCH][4], float (&sd)[2][SPR]) {
+    if (f_rb >= a.row_blocks) return;
+    // codes behind the matrix meet zeros of x, chunks behind the warp's are not multiplied: any word of the row will do there
+    const int first = (c_first + f_c) * (L4_CHUNK / 8) + t * WPL, last = a.words - WPL;
+#pragma unroll
+    for (int u = 0; u < L4_BATCH; ++u)
+#pragma unroll
+      for (int j = 0; j < GPC; ++j) {
+        const int at = min(first + u * (L4_CHUNK / 8) + j * 4 * WPL, last);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t* src = (r ? pc : pa) + at;
+          if (WPL == 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+            wd[r][u][0] = v.x; wd[r][u][1] = v.y; wd[r][u][2] = v.z; wd[r][u][3] = v.w;
+          } else if (WPL == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+            wd[r][u][2 * j] = v.x; wd[r][u][2 * j + 1] = v.y;
+          } else {
+            wd[r][u][j] = __ldg(src);
+          }
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < SPR; ++i) {
+      const int grp = (c_first + f_c) * GPC + 4 * i + t;
+      const bool in = grp < a.groups && f_c + (4 * i + t) / GPC < w_end;
+      sd[0][i] = in ? __half2float(sa[grp]) : 0.f;
+      sd[1][i] = in ? __half2float(sc[grp]) : 0.f;
+    }
+    f_c += L4_BATCH;
+    if (f_c >= w_end) {
+      f_c = w_first;
+      f_rb += clusters;
+      if (f_rb < a.row_blocks) rows_of(f_rb);
+    }
+  };
+  uint32_t w[2][2][L4_BATCH][4];           // [buffer][row][chunk][word]
+  float sv[2][2][SPR];                     // lane t: scale of group 4 i + t of the batch
   grid_launch_dependents();
-  grid_wait();
+  if (!a.early) grid_wait();
+  fetch(w[0], sv[0]);
+  if (a.early) grid_wait();
   // ---- x of this CTA's columns, in the order of the products
   {
-    const int words = (c_end - c_first) * (L4_CHUNK / 8);
-    for (int i = threadIdx.x; i < words * nn; i += L4_THREADS) {
-      const int n = i / words, w = i - n * words, k = c_first * L4_CHUNK + 8 * w;
-      const uint16_t* src = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(n0 + n) * a.ldx + k;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (a.vec_x && k + 8 <= a.K) v = *reinterpret_cast<const uint4*>(src);
-      else {
-        uint16_t* e = reinterpret_cast<uint16_t*>(&v);
+    const int words = wc * (L4_CHUNK / 8);
+    constexpr int U = NT >= 16 ? 8 : 4;
+    for (int i0 = threadIdx.x; i0 < words * nn; i0 += U * L4_THREADS) {
+      uint4 v[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j < a.K) e[j] = src[j];
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * L4_THREADS, n = i / words, k = c_first * L4_CHUNK + 8 * (i - n * words);
+        v[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < words * nn) {
+          const uint16_t* src = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(n0 + n) * a.ldx + k;
+          if (a.vec_x && k + 8 <= a.K) v[u] = *reinterpret_cast<const uint4*>(src);
+          else {
+            uint16_t* e = reinterpret_cast<uint16_t*>(&v[u]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (k + j < a.K) e[j] = src[j];
+          }
+        }
       }
-      *reinterpret_cast<uint4*>(l4_smem + l4_piece<NT>(l4_place<WPL>(w), n)) =
-          make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * L4_THREADS, n = i / words;
+        if (i < words * nn)
+          *reinterpret_cast<uint4*>(l4_smem + l4_piece<NT>(l4_place<WPL>(i - n * words), n)) =
+              make_uint4(__byte_perm(v[u].x, v[u].z, 0x5410), __byte_perm(v[u].x, v[u].z, 0x7632), __byte_perm(v[u].y, v[u].w, 0x5410),
+                         __byte_perm(v[u].y, v[u].w, 0x7632));
+      }
     }
   }
   __syncthreads();
-  const int wc = c_end - c_first, w_first = wc * kw / a.kwarps, w_end = wc * (kw + 1) / a.kwarps;      // this warp's chunks, CTA-relative
-  const int per = a.glu ? 8 : 16, cluster_id = blockIdx.x / a.splits, clusters = gridDim.x / a.splits;
-  for (int rb = cluster_id; rb < a.row_blocks; rb += clusters) {
-    const int r0 = (rb * rws + rw) * per;
-    // rows g and g + 8 of the unit
-    const int ra = r0 + g, rc = a.glu ? ra : r0 + 8 + g;
-    const uint32_t* pa = a.p[0] + static_cast<int64_t>(min(ra, a.N - 1)) * a.words;
-    const uint32_t* pc = (a.glu ? a.p[1] : a.p[0]) + static_cast<int64_t>(min(rc, a.N - 1)) * a.words;
-    const __half* sa = a.s[0] + static_cast<int64_t>(min(ra, a.N - 1)) * a.groups;
-    const __half* sc = (a.glu ? a.s[1] : a.s[0]) + static_cast<int64_t>(min(rc, a.N - 1)) * a.groups;
-    float acc[NB][4] = {};
-    uint32_t w[2][2][L4_BATCH][4];           // [buffer][row][chunk][word]
-    float sv[2][2][SPR];                     // lane t: scale of group 4 i + t of the batch
-    auto fetch = [&](int c, uint32_t (&wd)[2][L4_BATCH][4], float (&sd)[2][SPR]) {
+  float acc[NB][4] = {};
+  // where this lane's tokens' pieces start; columns of tokens that are not there may hold anything, they are not looked at
+  const unsigned char* xs[NB];
 #pragma unroll
-      for (int u = 0; u < L4_BATCH; ++u) {
-        const int word = (c_first + c + u) * (L4_CHUNK / 8);
+  for (int b = 0; b < NB; ++b) xs[b] = l4_smem + l4_piece<NT>(t, NT < 8 ? g % NT : 8 * b + g);
+  auto multiply = [&](int c, const uint32_t (&wd)[2][L4_BATCH][4], const float (&sd)[2][SPR]) {
+    const int base = c * (L4_CHUNK / 8) * NT * 16;
 #pragma unroll
-        for (int j = 0; j < GPC; ++j) {
-          const int at = word + (j * 4 + t) * WPL;
-          const bool in = c + u < w_end && at < a.words;
+    for (int u = 0; u < L4_BATCH; ++u) {
+      if (c + u >= w_end) break;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t* src = (r ? pc : pa) + at;
-            if (WPL == 4) {
-              const uint4 v = in ? __ldcs(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
-              wd[r][u][0] = v.x; wd[r][u][1] = v.y; wd[r][u][2] = v.z; wd[r][u][3] = v.w;
-            } else if (WPL == 2) {
-              const uint2 v = in ? __ldcs(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
-              wd[r][u][2 * j] = v.x; wd[r][u][2 * j + 1] = v.y;
-            } else {
-              wd[r][u][j] = in ? __ldg(src) : 0u;
-            }
-          }
-        }
-      }
+      for (int j = 0; j < GPC; ++j) {
+        float part[NB][4];
 #pragma unroll
-      for (int i = 0; i < SPR; ++i) {
-        const int grp = (c_first + c) * GPC + 4 * i + t;
-        const bool in = grp < a.groups && c + (4 * i + t) / GPC < w_end;
-        sd[0][i] = in ? __half2float(sa[grp]) : 0.f;
-        sd[1][i] = in ? __half2float(sc[grp]) : 0.f;
-      }
-    };
-    auto multiply = [&](int c, const uint32_t (&wd)[2][L4_BATCH][4], const float (&sd)[2][SPR]) {
-#pragma unroll
-      for (int u = 0; u < L4_BATCH; ++u) {
-        if (c + u >= w_end) break;
-#pragma unroll
-        for (int j = 0; j < GPC; ++j) {
-          float part[NB][4] = {};
-#pragma unroll
-          for (int v = 0; v < WPL; ++v) {
-            uint32_t qa[4], qc[4];
-            codes_to_pairs<XD>(wd[0][u][j * WPL + v], qa);
-            codes_to_pairs<XD>(wd[1][u][j * WPL + v], qc);
-            const uint32_t first[4] = {qa[0], qc[0], qa[1], qc[1]}, second[4] = {qa[2], qc[2], qa[3], qc[3]};
-            const int place = (c + u) * (L4_CHUNK / 8) + (j * WPL + v) * 4 + t;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              const int n = 8 * b + g;
-              uint4 xv = make_uint4(0u, 0u, 0u, 0u);
-              if (n < nn) xv = *reinterpret_cast<const uint4*>(l4_smem + l4_piece<NT>(place, n));
-              if (XD == BM_F16) {
-                mma_f16_16816(part[b], first, xv.x, xv.y);
-                mma_f16_16816(part[b], second, xv.z, xv.w);
-              } else {
-                mma_bf16_16816(part[b], first, xv.x, xv.y);
-                mma_bf16_16816(part[b], second, xv.z, xv.w);
-              }
-            }
-          }
-          const int q = u * GPC + j;
-          const float f0 = __shfl_sync(0xffffffffu, sd[0][q / 4], (lane & ~3) + q % 4), f1 = __shfl_sync(0xffffffffu, sd[1][q / 4], (lane & ~3) + q % 4);
+        for (int v = 0; v < WPL; ++v) {
+          uint32_t qa[4], qc[4];
+          codes_to_pairs<XD>(wd[0][u][j * WPL + v], qa);
+          codes_to_pairs<XD>(wd[1][u][j * WPL + v], qc);
+          const uint32_t first[4] = {qa[0], qc[0], qa[1], qc[1]}, second[4] = {qa[2], qc[2], qa[3], qc[3]};
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            acc[b][0] = fmaf(part[b][0], f0, acc[b][0]);
-            acc[b][1] = fmaf(part[b][1], f0, acc[b][1]);
-            acc[b][2] = fmaf(part[b][2], f1, acc[b][2]);
-            acc[b][3] = fmaf(part[b][3], f1, acc[b][3]);
+            const uint4 xv = *reinterpret_cast<const uint4*>(xs[b] + base + (u * (L4_CHUNK / 8) + (j * WPL + v) * 4) * NT * 16);
+            float (&p)[4] = part[b];
+            if (v == 0) mma_16816<XD>(p, first, xv.x, xv.y, 0.f, 0.f, 0.f, 0.f);
+            else mma_16816<XD>(p, first, xv.x, xv.y, p[0], p[1], p[2], p[3]);
+            mma_16816<XD>(p, second, xv.z, xv.w, p[0], p[1], p[2], p[3]);
           }
         }
+        const int q = u * GPC + j;
+        const float f0 = __shfl_sync(0xffffffffu, sd[0][q / 4], (lane & ~3) + q % 4), f1 = __shfl_sync(0xffffffffu, sd[1][q / 4], (lane & ~3) + q % 4);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          acc[b][0] = fmaf(part[b][0], f0, acc[b][0]);
+          acc[b][1] = fmaf(part[b][1], f0, acc[b][1]);
+          acc[b][2] = fmaf(part[b][2], f1, acc[b][2]);
+          acc[b][3] = fmaf(part[b][3], f1, acc[b][3]);
+        }
       }
-    };
-    fetch(w_first, w[0], sv[0]);
-    for (int c = w_first; c < w_end; c += 2 * L4_BATCH) {
-      if (c + L4_BATCH < w_end) fetch(c + L4_BATCH, w[1], sv[1]);
-      multiply(c, w[0], sv[0]);
-      if (c + L4_BATCH >= w_end) break;
-      if (c + 2 * L4_BATCH < w_end) fetch(c + 2 * L4_BATCH, w[0], sv[0]);
-      multiply(c + L4_BATCH, w[1], sv[1]);
     }
-    // ---- sums of the warps (and CTAs) that share the rows, then out
-    auto finish = [&](int row, int n, float v) {
-      const int64_t o = static_cast<int64_t>(n0 + n) * a.ldy + row;
-      if (a.row_gate) v *= a.row_gate[n0 + n];
-      if (a.residual) v += load_act(a.residual, a.y_dtype, static_cast<int64_t>(n0 + n) * a.N + row);
-      store_act(a.y, a.y_dtype, o, v);
-    };
+  };
+  // ---- sums of the warps (and CTAs) that share the rows, then out
+  auto finish_unit = [&](int rb) {
+    const int ra = (rb * rws + rw) * per + g, rc = ra + 8;
+    auto finish = [&](int row, int n, float v) { linear4_finish<XD>(a, n0 + n, row, v); };
     if (a.kwarps == 1 && a.splits == 1) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -224,7 +205,7 @@ __global__ void __launch_bounds__(L4_THREADS, 2) linear4_kernel(const __grid_con
             if (rc < a.N) finish(rc, n, acc[b][2 + i]);
           }
         }
-      continue;
+      return;
     }
     constexpr int COLS = 8 * NB, PART = 16 * COLS;       // floats of one warp's part: [row][token]
     float* mine = recv + (split * L4_WARPS + warp) * PART;
@@ -255,8 +236,28 @@ __global__ void __launch_bounds__(L4_THREADS, 2) linear4_kernel(const __grid_con
       }
     }
     if (a.splits == 1) __syncthreads();                  // the parts may be overwritten
+  };
+  int rb = cluster_id, c = w_first;
+  auto step = [&](uint32_t (&now)[2][L4_BATCH][4], float (&snow)[2][SPR], uint32_t (&next)[2][L4_BATCH][4], float (&snext)[2][SPR]) {
+    fetch(next, snext);
+    multiply(c, now, snow);
+    c += L4_BATCH;
+    if (c >= w_end) {
+      finish_unit(rb);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
+      c = w_first;
+      rb += clusters;
+    }
+    return rb < a.row_blocks;
+  };
+  while (step(w[0], sv[0], w[1], sv[1]) && step(w[1], sv[1], w[0], sv[0])) {
   }
 }
+
+constexpr int L4_TOKENS = 16;        // above, the tensor core's kernel
 
 static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
   const int chunks = (K + L4_CHUNK - 1) / L4_CHUNK, cols = nt < 8 ? 8 : nt;
@@ -291,17 +292,21 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
   a.words = (a.K + 31) / 32 * 4;
   a.groups = (a.K + group - 1) / group;
   a.vec_x = aligned16(a.x) && a.ldx % 8 == 0;
+  if (a.T > L4_TOKENS) {
+    const int rc = launch_linear4_tc(a, x_dtype, group, after, st);
+    if (rc != BM_ERR_UNSUPPORTED) return rc;
+  }
   const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK, units = (a.N + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
   int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32;
   // warps of a CTA, then CTAs of a cluster, share a row's columns until every SM has work
   a.kwarps = 1; a.splits = 1;
-  while (a.kwarps < 8 && a.kwarps < chunks && units * a.kwarps < 148 * 16) a.kwarps *= 2;
   while (nt > 8 && l4_smem_bytes(nt, a.K, 8, true) > 200 * 1024) nt /= 2;
   while (a.splits < 8 && l4_smem_bytes(nt, a.K, a.splits, true) > L4_SMEM) a.splits *= 2;
+  while (a.kwarps < 8 && 2 * a.kwarps * a.splits <= chunks && units * a.kwarps < 148 * 16) a.kwarps *= 2;
   BM_REQUIRE(l4_smem_bytes(nt, a.K, a.splits, true) <= 220 * 1024, BM_ERR_UNSUPPORTED, "linear4: %d columns are too many", a.K);
   const int rws = L4_WARPS / a.kwarps;
   a.row_blocks = (units + rws - 1) / rws;
-  const int most = 148 * 2 / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
+  const int most = 148 * l4_ctas(nt) / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
   const dim3 g(grid, (a.T + nt - 1) / nt);
   const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
   switch (nt) {
@@ -338,7 +343,7 @@ extern "C" int bm_linear4(const void* x, int dtype, const uint32_t* payload, con
   Linear4Args a{};
   a.p[0] = payload; a.s[0] = reinterpret_cast<const __half*>(scale);
   a.x = x; a.residual = residual; a.y = y;
-  a.T = T; a.K = K; a.N = N; a.ldx = K; a.ldy = N; a.y_dtype = dtype;
+  a.T = T; a.K = K; a.N = N; a.ldx = K; a.ldy = N;
   return linear4(a, dtype, group, AFTER_READS, static_cast<cudaStream_t>(stream));
 }
 
@@ -369,11 +374,11 @@ extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* g
   Linear4Args a{};
   a.p[0] = gate_payload; a.p[1] = up_payload;
   a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
-  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.y_dtype = dtype; a.glu = 1;
+  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1;
   if ((rc = linear4(a, dtype, group, AFTER_READS, st))) return rc;
   Linear4Args d{};
   d.p[0] = down_payload; d.s[0] = reinterpret_cast<const __half*>(down_scale);
   d.x = z; d.residual = residual; d.row_gate = token_gate_w ? gate : nullptr; d.y = y;
-  d.T = T; d.K = intermediate; d.N = hidden; d.ldx = ldz; d.ldy = hidden; d.y_dtype = dtype;
+  d.T = T; d.K = intermediate; d.N = hidden; d.ldx = ldz; d.ldy = hidden; d.early = 1;
   return linear4(d, dtype, group, AFTER_READS, st);
 }

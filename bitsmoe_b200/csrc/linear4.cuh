@@ -1,0 +1,63 @@
+// Products with 4-bit weights (linear4.cu, linear4_tc.cu).
+#pragma once
+
+#include "grouped.cuh"
+
+namespace bm {
+
+struct Linear4Args {
+  const uint32_t* p[2];        // codes [N, words]; GLU: gate and up
+  const __half* s[2];          // scales [N, groups]
+  const void* x;               // [T, ldx]
+  const void* residual;        // [T, N] of y's type, or null
+  const float* row_gate;       // factor per token, or null
+  void* y;                     // [T, ldy]
+  int T, K, N, ldx, ldy, words, groups;
+  int glu, vec_x, kwarps, splits, row_blocks, early;     // early: the launch before wrote none of the weights
+};
+
+// Eight codes -> four pairs (code i, code i + 4), i = 0 .. 3, as exact numbers -8 .. 7 of the type.
+template <int XD>
+__device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&q)[4]) {
+  if (XD == BM_F16) {
+    // 1024 + u and 1024 + 16 u are fp16 numbers with u in their low mantissa bits
+    const __half2 off = __float2half2_rn(1032.f), sixteenth = __float2half2_rn(0.0625f), minus72 = __float2half2_rn(-72.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h, w >>= 8) {
+      const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x64006400u;
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off), b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, minus72);
+      q[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
+      q[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  } else {
+    const __nv_bfloat162 off = __float2bfloat162_rn(136.f);       // 128 + u
+#pragma unroll
+    for (int i = 0; i < 4; ++i, w >>= 4) {
+      const uint32_t v = (w & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+      q[i] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+  }
+}
+
+template <int XD>
+__device__ __forceinline__ float load_x(const void* p, int64_t i) {
+  return XD == BM_F16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+template <int XD>
+__device__ __forceinline__ void store_x(void* p, int64_t i, float v) {
+  if (XD == BM_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+// What a finished sum becomes: times the token's gate, plus the residual.
+template <int XD>
+__device__ __forceinline__ void linear4_finish(const Linear4Args& a, int64_t token, int row, float v) {
+  if (a.row_gate) v *= a.row_gate[token];
+  if (a.residual) v += load_x<XD>(a.residual, token * a.N + row);
+  store_x<XD>(a.y, token * a.ldy + row, v);
+}
+
+// BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies.
+int launch_linear4_tc(const Linear4Args& a, int x_dtype, int group, LaunchAfter after, cudaStream_t st);
+
+}  // namespace bm

@@ -1,0 +1,288 @@
+// Products with 4-bit weights and group scales for more tokens than linear4_kernel streams the weights for, on tcgen05:
+//   y[t][n] = sum over groups of scale[n][g] * (sum over the group's columns of x[t][k] * q[n][k]),  q = code - 8
+//
+// The weights are the M operand (128 rows), the tokens the N operand (up to 128, in steps of 16).  Codes become exact 16-bit numbers of
+// x's type in shared memory; a group's products are summed by the tensor core into a tensor memory buffer of its own, and the epilogue
+// warps multiply each by the row's scale in fp32 as they add it to the sums they hold in registers -- a lane owns a row, so that its
+// scale is one value.  Nothing but y is rounded; weights rounded to 16 bits after scaling would put the result of an MLP twice as
+// far from the exact one as the rounding of its output does.
+//   warp 0       producer: codes (64 columns of 128 rows, 4 KB) twelve slices ahead, rows of x four slices ahead, as tiled copies
+//   warps 12-19  converters, two groups that take the slices in turn: codes -> pairs by mask and subtraction -> 128-byte swizzled rows
+//   warp 1       MMA issue: M = 128, N = the tile's tokens, K = 16; a commit per group of columns hands its buffer to the epilogue
+//   warps 4-11   epilogue: lane quarter, every other block of 16 tokens
+// With a gated pair the rows alternate between 16 gate rows and the 16 up rows that belong to them; lanes l and l + 16 exchange every
+// other token's sums at the end.  Waits are bounded.
+#include <cuda.h>
+
+#include <cstring>
+
+#include "linear4.cuh"
+#include "tc05.cuh"
+
+namespace bm {
+
+bool encode_map16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
+bool encode_map_bytes(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
+
+constexpr int LT_THREADS = 640, LT_EPI0 = 4, LT_EPI_WARPS = 8, LT_CONV0 = 12, LT_CONV_WARPS = 8, LT_ROWS = 128, LT_TOK = 128, LT_K = 64;
+constexpr int LT_P_BYTES = LT_ROWS * LT_K / 2, LT_A_BYTES = LT_ROWS * LT_K * 2, LT_B_BYTES = LT_TOK * LT_K * 2;
+constexpr int LT_PS = 12, LT_ABS = 4, LT_ACC = 4, LT_BOX = 32;       // slots of codes, stages of operands, accumulators; rows of x a copy
+constexpr int LT_SMEM = LT_PS * LT_P_BYTES + LT_ABS * (LT_A_BYTES + LT_B_BYTES) + 1024;
+
+struct LtParams {
+  CUtensorMap x, x8, p[2];     // x: 32 tokens or 8
+  Linear4Args a;
+  int slices, row_tiles, tok_tiles, tok_piece, parts, per_group;      // parts: groups as the slices make them; per_group: products of K = 16
+};
+
+__device__ __forceinline__ void lt_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(tc::smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+// K-major operand tile of 128-byte rows, 8-row groups 1024 bytes apart, 128-byte swizzle
+__device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <int XD, bool GLU>
+__global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_constant__ LtParams p) {
+  extern __shared__ unsigned char lt_raw[];
+  __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_ABS], a_ready[LT_ABS], ab_empty[LT_ABS], acc_full[LT_ACC], acc_empty[LT_ACC];
+  __shared__ uint32_t tmem_slot;
+  unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* const codes = smem + LT_ABS * (LT_A_BYTES + LT_B_BYTES);
+  const int warp = tc::warp_index(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < LT_PS; ++i) {
+      tc::mbar_init(&p_full[i], 1);
+      tc::mbar_init(&p_empty[i], LT_CONV_WARPS / 2);
+    }
+    for (int i = 0; i < LT_ABS; ++i) {
+      tc::mbar_init(&b_full[i], 1);
+      tc::mbar_init(&a_ready[i], LT_CONV_WARPS / 2);
+      tc::mbar_init(&ab_empty[i], 1);
+    }
+    for (int i = 0; i < LT_ACC; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], LT_EPI_WARPS);
+    }
+    tc::mbar_init_fence();
+  }
+  if (threadIdx.x == 96)
+    for (const CUtensorMap* m : {&p.x, &p.x8, &p.p[0], &p.p[1]}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+  if (warp == 2) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+  grid_launch_dependents();
+  grid_wait();
+  const int tiles = p.row_tiles * p.tok_tiles, grid = gridDim.x, mine = tiles > static_cast<int>(blockIdx.x) ? (tiles - blockIdx.x + grid - 1) / grid : 0;
+  const int total = mine * p.slices;           // slices of all of this CTA's tiles; neighbouring tiles share weight rows
+  auto tile_of = [&](int i, int& row0, int& tok0, int& n) {
+    const int tile = blockIdx.x + i * grid, rt = tile / p.tok_tiles;
+    row0 = rt * (GLU ? LT_ROWS / 2 : LT_ROWS);
+    tok0 = (tile - rt * p.tok_tiles) * p.tok_piece;
+    n = (min(p.tok_piece, p.a.T - tok0) + 15) & ~15;
+  };
+  bool ok = true;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer: two streams of copies, the codes ahead of the rows of x
+    int ps = 0, xs = 0, p_tile = 0, p_k = 0, x_tile = 0, x_k = 0, row0, tok0, n;
+    while (ok && xs < total) {
+      while (ok && ps < total && ps < xs + LT_PS) {
+        const int slot = ps % LT_PS;
+        if (ps >= LT_PS && !(ok = tc::mbar_wait(&p_empty[slot], (ps / LT_PS - 1) & 1))) break;
+        if (tc::elect_one()) {
+          tile_of(p_tile, row0, tok0, n);
+          unsigned char* to = codes + slot * LT_P_BYTES;
+          tc::mbar_expect_tx(&p_full[slot], LT_P_BYTES);
+          lt_load_2d(to, &p.p[0], p_k * (LT_K / 2), row0, &p_full[slot]);
+          lt_load_2d(to + LT_P_BYTES / 2, &p.p[GLU], p_k * (LT_K / 2), GLU ? row0 : row0 + LT_ROWS / 2, &p_full[slot]);
+        }
+        __syncwarp();
+        if (++p_k == p.slices) { p_k = 0; ++p_tile; }
+        ++ps;
+      }
+      const int st = xs % LT_ABS;
+      if (!ok || (xs >= LT_ABS && !(ok = tc::mbar_wait(&ab_empty[st], (xs / LT_ABS - 1) & 1)))) break;
+      if (tc::elect_one()) {
+        tile_of(x_tile, row0, tok0, n);
+        unsigned char* to = smem + st * (LT_A_BYTES + LT_B_BYTES) + LT_A_BYTES;
+        tc::mbar_expect_tx(&b_full[st], n * LT_K * 2);
+        int r = 0;
+        for (; r + LT_BOX <= n; r += LT_BOX) lt_load_2d(to + r * (LT_K * 2), &p.x, x_k * LT_K, tok0 + r, &b_full[st]);
+        for (; r < n; r += 8) lt_load_2d(to + r * (LT_K * 2), &p.x8, x_k * LT_K, tok0 + r, &b_full[st]);
+      }
+      __syncwarp();
+      if (++x_k == p.slices) { x_k = 0; ++x_tile; }
+      ++xs;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue
+    uint32_t acc = 0;                          // groups so far: buffer acc % LT_ACC
+    int s = 0;
+    for (int i = 0; i < mine && ok; ++i) {
+      int row0, tok0, n;
+      tile_of(i, row0, tok0, n);
+      const uint32_t idesc = XD == BM_F16 ? tc::idesc_f16(LT_ROWS, n) : tc::idesc_bf16(LT_ROWS, n);
+      int in_group = 0;
+      for (int k = 0; k < p.slices && ok; ++k, ++s) {
+        const int st = s % LT_ABS, ph = (s / LT_ABS) & 1;
+        if (!(ok = tc::mbar_wait(&b_full[st], ph) && tc::mbar_wait(&a_ready[st], ph))) break;
+        const uint32_t sa = tc::smem_u32(smem + st * (LT_A_BYTES + LT_B_BYTES));
+        const uint64_t ad = lt_desc(sa), bd = lt_desc(sa + LT_A_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < LT_K / 16; ++kk) {
+          const uint32_t buf = acc % LT_ACC;
+          if (in_group == 0 && acc >= LT_ACC && !(ok = tc::mbar_wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
+          tc::fence_after_sync();
+          const bool last = in_group + 1 == p.per_group || (k + 1 == p.slices && kk + 1 == LT_K / 16);
+          if (tc::elect_one()) {
+            tc::mma_f16(tmem_base + buf * LT_TOK, ad + 2 * kk, bd + 2 * kk, idesc, in_group > 0 ? 1u : 0u);
+            if (last) tc::mma_commit(&acc_full[buf]);
+            if (kk + 1 == LT_K / 16) tc::mma_commit(&ab_empty[st]);
+          }
+          __syncwarp();
+          in_group = last ? 0 : in_group + 1;
+          acc += last;
+        }
+      }
+    }
+  } else if (warp >= LT_CONV0) {
+    // ------------------------------------------------------------------ converters: a piece is 32 codes of a row
+    const int grp = (warp - LT_CONV0) / (LT_CONV_WARPS / 2), i = threadIdx.x - 32 * LT_CONV0 - grp * (16 * LT_CONV_WARPS);
+    for (int s = grp; s < total; s += 2) {
+      const int slot = s % LT_PS, st = s % LT_ABS;
+      if (!(ok = tc::mbar_wait(&p_full[slot], (s / LT_PS) & 1))) break;
+      uint4 w[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int piece = i + u * (16 * LT_CONV_WARPS), m = piece >> 1;
+        // row m of the operand: of a gated pair the gate rows come first among the codes
+        const int src = GLU ? ((m & 16) ? LT_ROWS / 2 : 0) + 16 * (m >> 5) + (m & 15) : m;
+        w[u] = *reinterpret_cast<const uint4*>(codes + slot * LT_P_BYTES + src * (LT_K / 2) + (piece & 1) * 16);
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_empty[slot]);
+      if (s >= LT_ABS && !(ok = tc::mbar_wait(&ab_empty[st], (s / LT_ABS - 1) & 1))) break;
+      unsigned char* const to = smem + st * (LT_A_BYTES + LT_B_BYTES);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int piece = i + u * (16 * LT_CONV_WARPS), m = piece >> 1;
+        const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t q[4];
+          codes_to_pairs<XD>(words[j], q);     // (0, 4) (1, 5) (2, 6) (3, 7) -> in order
+          *reinterpret_cast<uint4*>(to + m * 128 + (((4 * (piece & 1) + j) ^ (m & 7)) << 4)) =
+              make_uint4(__byte_perm(q[0], q[1], 0x5410), __byte_perm(q[2], q[3], 0x5410), __byte_perm(q[0], q[1], 0x7632), __byte_perm(q[2], q[3], 0x7632));
+        }
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&a_ready[st]);
+    }
+  } else if (warp >= LT_EPI0) {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - LT_EPI0) >> 2, up = GLU ? lane >> 4 : 0;
+    uint32_t acc = 0;
+    for (int i = 0; i < mine && ok; ++i) {
+      int row0, tok0, n;
+      tile_of(i, row0, tok0, n);
+      const int row = row0 + (GLU ? 16 * q + (lane & 15) : 32 * q + lane);
+      const __half* sc = p.a.s[up] + static_cast<int64_t>(min(row, p.a.N - 1)) * p.a.groups;
+      float sum[4][16] = {};
+      float f = __half2float(sc[0]);
+      for (int g = 0; g < p.parts; ++g, ++acc) {
+        const uint32_t buf = acc % LT_ACC;
+        // columns behind the matrix are zeros of x: what they are scaled by must only be finite
+        const float next = g + 1 < p.a.groups ? __half2float(sc[g + 1]) : 0.f;
+        if (!(ok = tc::mbar_wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
+        tc::fence_after_sync();
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + buf * LT_TOK;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int c0 = 16 * (half + 2 * b);
+          if (c0 >= n) break;
+          float v[16];
+          tc::tmem_ld16(at + c0, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[b][j] = fmaf(v[j], f, sum[b][j]);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+        f = next;
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int c0 = 16 * (half + 2 * b);
+        if (c0 >= n) break;
+        if (GLU) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? sum[b][j] : sum[b][j + 1], 16);
+            const int tok = tok0 + c0 + j + up;
+            if (tok < p.a.T && row < p.a.N) linear4_finish<XD>(p.a, tok, row, up ? silu_mul(other, sum[b][j + 1]) : silu_mul(sum[b][j], other));
+          }
+        } else if (row < p.a.N) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (tok0 + c0 + j < p.a.T) linear4_finish<XD>(p.a, tok0 + c0 + j, row, sum[b][j]);
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tc::tmem_dealloc(tmem_base, 512);
+}
+
+int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAfter after, cudaStream_t st) {
+  const Linear4Args& a = args;
+  if (a.ldx % 8 != 0 || !aligned16(a.x, a.p[0], a.p[1])) return BM_ERR_UNSUPPORTED;
+  LtParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.K), static_cast<cuuint64_t>(a.T)}, strides[1] = {static_cast<cuuint64_t>(a.ldx) * 2};
+    const cuuint32_t box[2] = {LT_K, LT_BOX}, box8[2] = {LT_K, 8};
+    if (!encode_map16(&p.x, a.x, 2, dims, strides, box) || !encode_map16(&p.x8, a.x, 2, dims, strides, box8)) return BM_ERR_UNSUPPORTED;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.words) * 4, static_cast<cuuint64_t>(a.N)}, strides[1] = {static_cast<cuuint64_t>(a.words) * 4};
+    const cuuint32_t box[2] = {LT_K / 2, LT_ROWS / 2};
+    if (!encode_map_bytes(&p.p[i], a.p[a.glu ? i : 0], 2, dims, strides, box)) return BM_ERR_UNSUPPORTED;
+  }
+  p.slices = (a.K + LT_K - 1) / LT_K;
+  p.per_group = group / 16;
+  p.parts = (p.slices * (LT_K / 16) + p.per_group - 1) / p.per_group;
+  p.row_tiles = (a.N + (a.glu ? LT_ROWS / 2 : LT_ROWS) - 1) / (a.glu ? LT_ROWS / 2 : LT_ROWS);
+  const int pieces = (a.T + LT_TOK - 1) / LT_TOK;
+  p.tok_piece = ((a.T + pieces - 1) / pieces + 15) & ~15;
+  p.tok_tiles = (a.T + p.tok_piece - 1) / p.tok_piece;
+  if (static_cast<int64_t>(p.row_tiles) * p.tok_tiles * p.slices > 0x3fffffff) return BM_ERR_UNSUPPORTED;
+  static PerDeviceOnce once;
+  static int sms[MAX_DEVICES];
+  int dev = -1;
+  BM_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= MAX_DEVICES) return BM_ERR_UNSUPPORTED;
+  if (!once.is_done(dev)) {
+    for (auto* kernel : {linear4_tc_kernel<BM_F16, false>, linear4_tc_kernel<BM_F16, true>, linear4_tc_kernel<BM_BF16, false>, linear4_tc_kernel<BM_BF16, true>})
+      BM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM));
+    BM_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
+    once.mark(dev);
+  }
+  const int tiles = p.row_tiles * p.tok_tiles, grid = tiles < sms[dev] ? tiles : sms[dev];
+  auto* kernel = x_dtype == BM_F16 ? (a.glu ? linear4_tc_kernel<BM_F16, true> : linear4_tc_kernel<BM_F16, false>)
+                                   : (a.glu ? linear4_tc_kernel<BM_BF16, true> : linear4_tc_kernel<BM_BF16, false>);
+  BM_CUDA(launch_after(after, 1, kernel, dim3(grid), LT_THREADS, LT_SMEM, st, p));
+  BM_LAUNCH_CHECK("linear4_tc_kernel");
+  return BM_OK;
+}
+
+}  // namespace bm
