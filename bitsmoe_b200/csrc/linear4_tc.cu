@@ -6,7 +6,7 @@
 // warps multiply each by the row's scale in fp32 as they add it to the sums they hold in registers -- a lane owns a row, so that its
 // scale is one value.  Nothing but y is rounded; weights rounded to 16 bits after scaling would put the result of an MLP twice as
 // far from the exact one as the rounding of its output does.
-//   warp 0       producer: codes (64 columns of 128 rows, 4 KB) twelve slices ahead, rows of x four slices ahead, as tiled copies
+//   warps 0, 3   producers: codes (64 columns of 128 rows, 4 KB) twelve slices ahead; rows of x four slices ahead, as tiled copies
 //   warps 12-19  converters, two groups that take the slices in turn: codes -> pairs by mask and subtraction -> 128-byte swizzled rows
 //   warp 1       MMA issue: M = 128, N = the tile's tokens, K = 16; a commit per group of columns hands its buffer to the epilogue
 //   warps 4-11   epilogue: lane quarter, every other block of 16 tokens
@@ -89,36 +89,41 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   bool ok = true;
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ producer: two streams of copies, the codes ahead of the rows of x
-    int ps = 0, xs = 0, p_tile = 0, p_k = 0, x_tile = 0, x_k = 0, row0, tok0, n;
-    while (ok && xs < total) {
-      while (ok && ps < total && ps < xs + LT_PS) {
-        const int slot = ps % LT_PS;
-        if (ps >= LT_PS && !(ok = tc::mbar_wait(&p_empty[slot], (ps / LT_PS - 1) & 1))) break;
+    // ------------------------------------------------------------------ codes, as far ahead as there are slots
+    int slot = 0, ph = 1;
+    for (int i = 0; i < mine && ok; ++i) {
+      int row0, tok0, n;
+      tile_of(i, row0, tok0, n);
+      for (int k = 0; k < p.slices; ++k) {
+        if (!(ok = tc::mbar_wait(&p_empty[slot], ph))) break;
         if (tc::elect_one()) {
-          tile_of(p_tile, row0, tok0, n);
           unsigned char* to = codes + slot * LT_P_BYTES;
           tc::mbar_expect_tx(&p_full[slot], LT_P_BYTES);
-          lt_load_2d(to, &p.p[0], p_k * (LT_K / 2), row0, &p_full[slot]);
-          lt_load_2d(to + LT_P_BYTES / 2, &p.p[GLU], p_k * (LT_K / 2), GLU ? row0 : row0 + LT_ROWS / 2, &p_full[slot]);
+          lt_load_2d(to, &p.p[0], k * (LT_K / 2), row0, &p_full[slot]);
+          lt_load_2d(to + LT_P_BYTES / 2, &p.p[GLU], k * (LT_K / 2), GLU ? row0 : row0 + LT_ROWS / 2, &p_full[slot]);
         }
         __syncwarp();
-        if (++p_k == p.slices) { p_k = 0; ++p_tile; }
-        ++ps;
+        if (++slot == LT_PS) { slot = 0; ph ^= 1; }
       }
-      const int st = xs % LT_ABS;
-      if (!ok || (xs >= LT_ABS && !(ok = tc::mbar_wait(&ab_empty[st], (xs / LT_ABS - 1) & 1)))) break;
-      if (tc::elect_one()) {
-        tile_of(x_tile, row0, tok0, n);
-        unsigned char* to = smem + st * (LT_A_BYTES + LT_B_BYTES) + LT_A_BYTES;
-        tc::mbar_expect_tx(&b_full[st], n * LT_K * 2);
-        int r = 0;
-        for (; r + LT_BOX <= n; r += LT_BOX) lt_load_2d(to + r * (LT_K * 2), &p.x, x_k * LT_K, tok0 + r, &b_full[st]);
-        for (; r < n; r += 8) lt_load_2d(to + r * (LT_K * 2), &p.x8, x_k * LT_K, tok0 + r, &b_full[st]);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ rows of x
+    int st = 0, ph = 1;
+    for (int i = 0; i < mine && ok; ++i) {
+      int row0, tok0, n;
+      tile_of(i, row0, tok0, n);
+      for (int k = 0; k < p.slices; ++k) {
+        if (!(ok = tc::mbar_wait(&ab_empty[st], ph))) break;
+        if (tc::elect_one()) {
+          unsigned char* to = smem + st * (LT_A_BYTES + LT_B_BYTES) + LT_A_BYTES;
+          tc::mbar_expect_tx(&b_full[st], n * LT_K * 2);
+          int r = 0;
+          for (; r + LT_BOX <= n; r += LT_BOX) lt_load_2d(to + r * (LT_K * 2), &p.x, k * LT_K, tok0 + r, &b_full[st]);
+          for (; r < n; r += 8) lt_load_2d(to + r * (LT_K * 2), &p.x8, k * LT_K, tok0 + r, &b_full[st]);
+        }
+        __syncwarp();
+        if (++st == LT_ABS) { st = 0; ph ^= 1; }
       }
-      __syncwarp();
-      if (++x_k == p.slices) { x_k = 0; ++x_tile; }
-      ++xs;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
@@ -165,8 +170,6 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
         const int src = GLU ? ((m & 16) ? LT_ROWS / 2 : 0) + 16 * (m >> 5) + (m & 15) : m;
         w[u] = *reinterpret_cast<const uint4*>(codes + slot * LT_P_BYTES + src * (LT_K / 2) + (piece & 1) * 16);
       }
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&p_empty[slot]);
       if (s >= LT_ABS && !(ok = tc::mbar_wait(&ab_empty[st], (s / LT_ABS - 1) & 1))) break;
       unsigned char* const to = smem + st * (LT_A_BYTES + LT_B_BYTES);
 #pragma unroll
@@ -183,7 +186,12 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       }
       tc::fence_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&a_ready[st]);
+      // the codes' slot is given back here, where what was read of it has been stored: the compiler may move the loads down to their use,
+      // past an arrival that stands between the two (it did: rows of the slice twelve later, once the epilogue was fast enough to wait)
+      if (lane == 0) {
+        tc::mbar_arrive(&p_empty[slot]);
+        tc::mbar_arrive(&a_ready[st]);
+      }
     }
   } else if (warp >= LT_EPI0) {
     // ------------------------------------------------------------------ epilogue
@@ -195,27 +203,38 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       const int row = row0 + (GLU ? 16 * q + (lane & 15) : 32 * q + lane);
       const __half* sc = p.a.s[up] + static_cast<int64_t>(min(row, p.a.N - 1)) * p.a.groups;
       float sum[4][16] = {};
-      float f = __half2float(sc[0]);
-      for (int g = 0; g < p.parts; ++g, ++acc) {
-        const uint32_t buf = acc % LT_ACC;
-        // columns behind the matrix are zeros of x: what they are scaled by must only be finite
-        const float next = g + 1 < p.a.groups ? __half2float(sc[g + 1]) : 0.f;
-        if (!(ok = tc::mbar_wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
-        tc::fence_after_sync();
-        const uint32_t at = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + buf * LT_TOK;
+      // scales four groups ahead; columns behind the matrix are zeros of x, what they are scaled by must only be finite
+      uint32_t ahead[4];
+      auto load_scales = [&](int g0) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int c0 = 16 * (half + 2 * b);
-          if (c0 >= n) break;
-          float v[16];
-          tc::tmem_ld16(at + c0, v);
+        for (int j = 0; j < 4; ++j) ahead[j] = g0 + j < p.a.groups ? __ldg(reinterpret_cast<const unsigned short*>(sc) + g0 + j) : 0u;
+      };
+      load_scales(0);
+      for (int g0 = 0; g0 < p.parts && ok; g0 += 4) {
+        const uint32_t now[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
+        load_scales(g0 + 4);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) sum[b][j] = fmaf(v[j], f, sum[b][j]);
+        for (int j = 0; j < 4; ++j) {
+          if (g0 + j >= p.parts) break;
+          const uint32_t buf = acc % LT_ACC;
+          if (!(ok = tc::mbar_wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
+          tc::fence_after_sync();
+          const uint32_t at = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + buf * LT_TOK;
+          const float f = __half2float(__ushort_as_half(static_cast<unsigned short>(now[j])));
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int c0 = 16 * (half + 2 * b);
+            if (c0 >= n) break;
+            float v[16];
+            tc::tmem_ld16(at + c0, v);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) sum[b][c] = fmaf(v[c], f, sum[b][c]);
+          }
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+          ++acc;
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
-        f = next;
       }
       if (!ok) break;
 #pragma unroll
