@@ -6,10 +6,11 @@
 // warps multiply each by the row's scale in fp32 as they add it to the sums they hold in registers -- a lane owns a row, so that its
 // scale is one value.  Nothing but y is rounded; weights rounded to 16 bits after scaling would put the result of an MLP twice as
 // far from the exact one as the rounding of its output does.
-//   warps 0, 3   producers: codes (64 columns of 128 rows, 4 KB) twelve slices ahead; rows of x four slices ahead, as tiled copies
+//   warps 0, 3   producers: codes (64 columns of 128 rows, 4 KB) twelve slices ahead; rows of x six to twelve, as tiled copies
 //   warps 12-19  converters, two groups that take the slices in turn: codes -> pairs by mask and subtraction -> 128-byte swizzled rows
 //   warp 1       MMA issue: M = 128, N = the tile's tokens, K = 16; a commit per group of columns hands its buffer to the epilogue
 //   warps 4-11   epilogue: lane quarter, every other block of 16 tokens
+// Where there are few tiles, clusters of CTAs share a tile's columns and add their sums up in the first one's shared memory, in order.
 // With a gated pair the rows alternate between 16 gate rows and the 16 up rows that belong to them; lanes l and l + 16 exchange every
 // other token's sums at the end.  Waits are bounded.
 #include <cuda.h>
@@ -26,13 +27,14 @@ bool encode_map_bytes(CUtensorMap* map, const void* base, int rank, const cuuint
 
 constexpr int LT_THREADS = 640, LT_EPI0 = 4, LT_EPI_WARPS = 8, LT_CONV0 = 12, LT_CONV_WARPS = 8, LT_ROWS = 128, LT_TOK = 128, LT_K = 64;
 constexpr int LT_P_BYTES = LT_ROWS * LT_K / 2, LT_A_BYTES = LT_ROWS * LT_K * 2, LT_B_BYTES = LT_TOK * LT_K * 2;
-constexpr int LT_PS = 12, LT_ABS = 4, LT_ACC = 4, LT_BOX = 32;       // slots of codes, stages of operands, accumulators; rows of x a copy
-constexpr int LT_SMEM = LT_PS * LT_P_BYTES + LT_ABS * (LT_A_BYTES + LT_B_BYTES) + 1024;
+constexpr int LT_PS = 12, LT_AS = 4, LT_BS = 12, LT_ACC = 4, LT_BOX = 32;       // slots of codes, stages of weights and (at most) of x, accumulators; rows of x a copy
+constexpr int LT_B_RING = 6 * LT_B_BYTES;
+constexpr int LT_SMEM = LT_PS * LT_P_BYTES + LT_AS * LT_A_BYTES + LT_B_RING + 1024;
 
 struct LtParams {
   CUtensorMap x, x8, p[2];     // x: 32 tokens or 8
   Linear4Args a;
-  int slices, row_tiles, tok_tiles, tok_piece, parts, per_group;      // parts: groups as the slices make them; per_group: products of K = 16
+  int splits, slices, row_tiles, tok_tiles, tok_piece, per_group;      // splits: CTAs that share a tile's columns; per_group: products of K = 16
 };
 
 __device__ __forceinline__ void lt_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -48,20 +50,23 @@ __device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
 template <int XD, bool GLU>
 __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_constant__ LtParams p) {
   extern __shared__ unsigned char lt_raw[];
-  __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_ABS], a_ready[LT_ABS], ab_empty[LT_ABS], acc_full[LT_ACC], acc_empty[LT_ACC];
+  __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_BS], b_empty[LT_BS], a_ready[LT_AS], a_empty[LT_AS], acc_full[LT_ACC], acc_empty[LT_ACC];
   __shared__ uint32_t tmem_slot;
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char* const codes = smem + LT_ABS * (LT_A_BYTES + LT_B_BYTES);
+  unsigned char *const b_ring = smem + LT_AS * LT_A_BYTES, *const codes = b_ring + LT_B_RING;
   const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < LT_PS; ++i) {
       tc::mbar_init(&p_full[i], 1);
       tc::mbar_init(&p_empty[i], LT_CONV_WARPS / 2);
     }
-    for (int i = 0; i < LT_ABS; ++i) {
+    for (int i = 0; i < LT_BS; ++i) {
       tc::mbar_init(&b_full[i], 1);
+      tc::mbar_init(&b_empty[i], 1);
+    }
+    for (int i = 0; i < LT_AS; ++i) {
       tc::mbar_init(&a_ready[i], LT_CONV_WARPS / 2);
-      tc::mbar_init(&ab_empty[i], 1);
+      tc::mbar_init(&a_empty[i], 1);
     }
     for (int i = 0; i < LT_ACC; ++i) {
       tc::mbar_init(&acc_full[i], 1);
@@ -78,14 +83,18 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   const uint32_t tmem_base = tmem_slot;
   grid_launch_dependents();
   grid_wait();
-  const int tiles = p.row_tiles * p.tok_tiles, grid = gridDim.x, mine = tiles > static_cast<int>(blockIdx.x) ? (tiles - blockIdx.x + grid - 1) / grid : 0;
-  const int total = mine * p.slices;           // slices of all of this CTA's tiles; neighbouring tiles share weight rows
+  // tiles of this CTA (neighbours share weight rows), and its slices of their columns: all, or a share that starts with a group
+  const int rank = blockIdx.x % p.splits, first = blockIdx.x / p.splits, grid = gridDim.x / p.splits, tiles = p.row_tiles * p.tok_tiles;
+  const int mine = tiles > first ? (tiles - first + grid - 1) / grid : 0;
+  const int k_first = p.slices * rank / p.splits & ~1, k_end = rank + 1 < p.splits ? p.slices * (rank + 1) / p.splits & ~1 : p.slices;
+  const int slices = k_end - k_first, total = mine * slices;
   auto tile_of = [&](int i, int& row0, int& tok0, int& n) {
-    const int tile = blockIdx.x + i * grid, rt = tile / p.tok_tiles;
+    const int tile = first + i * grid, rt = tile / p.tok_tiles;
     row0 = rt * (GLU ? LT_ROWS / 2 : LT_ROWS);
     tok0 = (tile - rt * p.tok_tiles) * p.tok_piece;
     n = (min(p.tok_piece, p.a.T - tok0) + 15) & ~15;
   };
+  const int b_bytes = p.tok_piece * LT_K * 2, b_stages = min(LT_B_RING / b_bytes, LT_BS);
   bool ok = true;
 
   if (warp == 0) {
@@ -94,7 +103,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
     for (int i = 0; i < mine && ok; ++i) {
       int row0, tok0, n;
       tile_of(i, row0, tok0, n);
-      for (int k = 0; k < p.slices; ++k) {
+      for (int k = k_first; k < k_end; ++k) {
         if (!(ok = tc::mbar_wait(&p_empty[slot], ph))) break;
         if (tc::elect_one()) {
           unsigned char* to = codes + slot * LT_P_BYTES;
@@ -112,55 +121,65 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
     for (int i = 0; i < mine && ok; ++i) {
       int row0, tok0, n;
       tile_of(i, row0, tok0, n);
-      for (int k = 0; k < p.slices; ++k) {
-        if (!(ok = tc::mbar_wait(&ab_empty[st], ph))) break;
+      for (int k = k_first; k < k_end; ++k) {
+        if (!(ok = tc::mbar_wait(&b_empty[st], ph))) break;
         if (tc::elect_one()) {
-          unsigned char* to = smem + st * (LT_A_BYTES + LT_B_BYTES) + LT_A_BYTES;
+          unsigned char* to = b_ring + st * b_bytes;
           tc::mbar_expect_tx(&b_full[st], n * LT_K * 2);
           int r = 0;
           for (; r + LT_BOX <= n; r += LT_BOX) lt_load_2d(to + r * (LT_K * 2), &p.x, k * LT_K, tok0 + r, &b_full[st]);
           for (; r < n; r += 8) lt_load_2d(to + r * (LT_K * 2), &p.x8, k * LT_K, tok0 + r, &b_full[st]);
         }
         __syncwarp();
-        if (++st == LT_ABS) { st = 0; ph ^= 1; }
+        if (++st == b_stages) { st = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
     uint32_t acc = 0;                          // groups so far: buffer acc % LT_ACC
-    int s = 0;
+    const int run = min(p.per_group, LT_K / 16);
+    int s = 0, bs = 0, b_ph = 0;
     for (int i = 0; i < mine && ok; ++i) {
       int row0, tok0, n;
       tile_of(i, row0, tok0, n);
       const uint32_t idesc = XD == BM_F16 ? tc::idesc_f16(LT_ROWS, n) : tc::idesc_bf16(LT_ROWS, n);
       int in_group = 0;
-      for (int k = 0; k < p.slices && ok; ++k, ++s) {
-        const int st = s % LT_ABS, ph = (s / LT_ABS) & 1;
-        if (!(ok = tc::mbar_wait(&b_full[st], ph) && tc::mbar_wait(&a_ready[st], ph))) break;
-        const uint32_t sa = tc::smem_u32(smem + st * (LT_A_BYTES + LT_B_BYTES));
-        const uint64_t ad = lt_desc(sa), bd = lt_desc(sa + LT_A_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < LT_K / 16; ++kk) {
+      for (int k = 0; k < slices && ok; ++k, ++s) {
+        const int st = s % LT_AS;
+        if (!(ok = tc::mbar_wait(&b_full[bs], b_ph) && tc::mbar_wait(&a_ready[st], (s / LT_AS) & 1))) break;
+        const uint64_t ad = lt_desc(tc::smem_u32(smem + st * LT_A_BYTES)), bd = lt_desc(tc::smem_u32(b_ring + bs * b_bytes));
+        // the slice's products of one group at a time: four, or two and two
+        for (int kk = 0; kk < LT_K / 16; kk += run) {
           const uint32_t buf = acc % LT_ACC;
           if (in_group == 0 && acc >= LT_ACC && !(ok = tc::mbar_wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
           tc::fence_after_sync();
-          const bool last = in_group + 1 == p.per_group || (k + 1 == p.slices && kk + 1 == LT_K / 16);
+          const bool last = in_group + run == p.per_group || (k + 1 == slices && kk + run == LT_K / 16);
           if (tc::elect_one()) {
-            tc::mma_f16(tmem_base + buf * LT_TOK, ad + 2 * kk, bd + 2 * kk, idesc, in_group > 0 ? 1u : 0u);
+            const uint32_t d = tmem_base + buf * LT_TOK;
+            tc::mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, in_group > 0 ? 1u : 0u);
+            tc::mma_f16(d, ad + 2 * kk + 2, bd + 2 * kk + 2, idesc, 1u);
+            if (run == 4) {
+              tc::mma_f16(d, ad + 4, bd + 4, idesc, 1u);
+              tc::mma_f16(d, ad + 6, bd + 6, idesc, 1u);
+            }
             if (last) tc::mma_commit(&acc_full[buf]);
-            if (kk + 1 == LT_K / 16) tc::mma_commit(&ab_empty[st]);
+            if (kk + run == LT_K / 16) {
+              tc::mma_commit(&a_empty[st]);
+              tc::mma_commit(&b_empty[bs]);
+            }
           }
           __syncwarp();
-          in_group = last ? 0 : in_group + 1;
+          in_group = last ? 0 : in_group + run;
           acc += last;
         }
+        if (++bs == b_stages) { bs = 0; b_ph ^= 1; }
       }
     }
   } else if (warp >= LT_CONV0) {
     // ------------------------------------------------------------------ converters: a piece is 32 codes of a row
     const int grp = (warp - LT_CONV0) / (LT_CONV_WARPS / 2), i = threadIdx.x - 32 * LT_CONV0 - grp * (16 * LT_CONV_WARPS);
     for (int s = grp; s < total; s += 2) {
-      const int slot = s % LT_PS, st = s % LT_ABS;
+      const int slot = s % LT_PS, st = s % LT_AS;
       if (!(ok = tc::mbar_wait(&p_full[slot], (s / LT_PS) & 1))) break;
       uint4 w[2];
 #pragma unroll
@@ -170,8 +189,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
         const int src = GLU ? ((m & 16) ? LT_ROWS / 2 : 0) + 16 * (m >> 5) + (m & 15) : m;
         w[u] = *reinterpret_cast<const uint4*>(codes + slot * LT_P_BYTES + src * (LT_K / 2) + (piece & 1) * 16);
       }
-      if (s >= LT_ABS && !(ok = tc::mbar_wait(&ab_empty[st], (s / LT_ABS - 1) & 1))) break;
-      unsigned char* const to = smem + st * (LT_A_BYTES + LT_B_BYTES);
+      if (s >= LT_AS && !(ok = tc::mbar_wait(&a_empty[st], (s / LT_AS - 1) & 1))) break;
+      unsigned char* const to = smem + st * LT_A_BYTES;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int piece = i + u * (16 * LT_CONV_WARPS), m = piece >> 1;
@@ -209,13 +228,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < 4; ++j) ahead[j] = g0 + j < p.a.groups ? __ldg(reinterpret_cast<const unsigned short*>(sc) + g0 + j) : 0u;
       };
-      load_scales(0);
-      for (int g0 = 0; g0 < p.parts && ok; g0 += 4) {
+      const int g_first = k_first * (LT_K / 16) / p.per_group, g_end = g_first + (slices * (LT_K / 16) + p.per_group - 1) / p.per_group;
+      load_scales(g_first);
+      for (int g0 = g_first; g0 < g_end && ok; g0 += 4) {
         const uint32_t now[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
         load_scales(g0 + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (g0 + j >= p.parts) break;
+          if (g0 + j >= g_end) break;
           const uint32_t buf = acc % LT_ACC;
           if (!(ok = tc::mbar_wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
           tc::fence_after_sync();
@@ -235,6 +255,31 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
           if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
           ++acc;
         }
+      }
+      if (p.splits > 1) {
+        // (one tile a CTA) the sums meet in the first CTA's shared memory, whose rings nothing uses any more behind the first barrier
+        const int me = threadIdx.x - 32 * LT_EPI0;
+        tc::cluster_arrive();
+        tc::cluster_wait();
+        if (rank > 0)
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int c = 0; c < 16; c += 4)
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(tc::cluster_map(tc::smem_u32(smem) + (((rank - 1) * 16 + 4 * b + c / 4) * 32 * LT_EPI_WARPS + me) * 16, 0)),
+                           "f"(sum[b][c]), "f"(sum[b][c + 1]), "f"(sum[b][c + 2]), "f"(sum[b][c + 3])
+                           : "memory");
+        tc::cluster_arrive();
+        tc::cluster_wait();
+        if (rank > 0) break;
+        for (int r = 1; r < p.splits; ++r)
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(smem + (((r - 1) * 16 + 4 * b + c / 4) * 32 * LT_EPI_WARPS + me) * 16);
+              sum[b][c] += v.x; sum[b][c + 1] += v.y; sum[b][c + 2] += v.z; sum[b][c + 3] += v.w;
+            }
       }
       if (!ok) break;
 #pragma unroll
@@ -256,6 +301,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       }
     }
   }
+  if (p.splits > 1 && (warp < LT_EPI0 || warp >= LT_CONV0))
+    for (int i = 0; i < 2; ++i) {
+      tc::cluster_arrive();
+      tc::cluster_wait();
+    }
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 2) tc::tmem_dealloc(tmem_base, 512);
@@ -279,7 +329,6 @@ int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAft
   }
   p.slices = (a.K + LT_K - 1) / LT_K;
   p.per_group = group / 16;
-  p.parts = (p.slices * (LT_K / 16) + p.per_group - 1) / p.per_group;
   p.row_tiles = (a.N + (a.glu ? LT_ROWS / 2 : LT_ROWS) - 1) / (a.glu ? LT_ROWS / 2 : LT_ROWS);
   const int pieces = (a.T + LT_TOK - 1) / LT_TOK;
   p.tok_piece = ((a.T + pieces - 1) / pieces + 15) & ~15;
@@ -296,10 +345,15 @@ int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAft
     BM_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     once.mark(dev);
   }
-  const int tiles = p.row_tiles * p.tok_tiles, grid = tiles < sms[dev] ? tiles : sms[dev];
+  // few tiles: clusters of two or four CTAs share the columns of one (a cluster of four leaves a few SMs of a group unused)
+  const int tiles = p.row_tiles * p.tok_tiles;
+  p.splits = 1;
+  if (tiles * 4 <= sms[dev] * 7 / 8 && p.slices >= 8) p.splits = 4;
+  else if (tiles * 2 <= sms[dev] && p.slices >= 4) p.splits = 2;
+  const int grid = p.splits > 1 ? tiles * p.splits : tiles < sms[dev] ? tiles : sms[dev];
   auto* kernel = x_dtype == BM_F16 ? (a.glu ? linear4_tc_kernel<BM_F16, true> : linear4_tc_kernel<BM_F16, false>)
                                    : (a.glu ? linear4_tc_kernel<BM_BF16, true> : linear4_tc_kernel<BM_BF16, false>);
-  BM_CUDA(launch_after(after, 1, kernel, dim3(grid), LT_THREADS, LT_SMEM, st, p));
+  BM_CUDA(launch_after(after, p.splits, kernel, dim3(grid), LT_THREADS, LT_SMEM, st, p));
   BM_LAUNCH_CHECK("linear4_tc_kernel");
   return BM_OK;
 }
