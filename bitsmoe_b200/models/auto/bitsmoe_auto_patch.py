@@ -24,7 +24,7 @@ from __future__ import annotations
 import copy
 import os
 from types import SimpleNamespace
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import torch
 import torch.nn as nn
@@ -36,6 +36,7 @@ from bitsmoe_b200.models.qwen3moe.bitsmoe_block import BitsMoE_Qwen3MoeSparseMoe
 from bitsmoe_b200.models.qwen3moe.bitsmoe_mlp import BitsMoE_Qwen3MoeMLP
 from bitsmoe_b200.models.qwen3next.bitsmoe_block import BitsMoE_Qwen3NextSparseMoeBlock
 from bitsmoe_b200.models.qwen3next.bitsmoe_mlp import BitsMoE_Qwen3NextMLP
+from bitsmoe_b200.quant.linear4 import Linear4
 
 # un-quantised ("super") experts per layer of the released checkpoints (bitsmoe_auto_patch.py:42-46)
 _SUPER_EXPERTS_BY_MODEL: Dict[str, Dict[int, List[int]]] = {
@@ -182,6 +183,26 @@ def patch_bitsmoe_inplace(model, bitsmoe_model_type: str, packed_state: Optional
         setattr(layer, attr, block)
     setattr(model, "_bitsmoe_packed_expert_total", int(total))
     return total
+
+
+def quantize_dense_inplace(model, group_size: int = 128, projections: Sequence[str] = ("q_proj", "k_proj", "v_proj", "o_proj"),
+                           shared_experts: bool = True) -> int:
+    """Holds dense weights of a patched model in 4 bits: the bias-free Linears of its decoder layers that are named in ``projections``
+    (outside the MoE blocks), and the MoE blocks' shared experts.  Returns how many Linears were replaced.  The routed experts are packed
+    already, so these 16-bit matrices are most of what a decode step reads; routers, embeddings and the output layer stay as they are."""
+    n, inside = 0, set()
+    for block in (m for m in model.modules() if isinstance(m, BitsMoE_BaseSparseMoeBlock)):
+        inside.update(id(m) for m in block.modules())
+        if shared_experts:
+            n += block.quantize_shared_experts(group_size)
+    for layer in model.model.layers:
+        for parent in list(layer.modules()):
+            for name in projections:
+                lin = parent._modules.get(name)
+                if id(parent) not in inside and isinstance(lin, nn.Linear) and lin.bias is None:
+                    setattr(parent, name, Linear4.from_linear(lin, group_size))
+                    n += 1
+    return n
 
 
 def prepare_bitsmoe_runtime(model, warmup: Optional[bool] = None) -> int:

@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from bitsmoe_b200.algorithms import _HAS_MLP_FORWARD_CUDA, mlp_forward_cuda
+from bitsmoe_b200.quant.linear4 import Linear4
 
 _FIELDS = ("payload", "rank_idx", "tile_meta", "slab_meta", "scale", "s")
 _TAGS = ("gate", "up", "down")
@@ -37,6 +38,8 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         for key in self._SHARED_BASIS_BUFFER_KEYS:
             self.register_buffer(key, torch.empty(0, dtype=torch.float16), persistent=True)
         self._super_expert_items: List[Tuple[int, nn.Module]] = []
+        self._super_weights: Optional[Tuple[torch.Tensor, torch.Tensor]] = None     # gate and up rows [E, 2I, H], down [E, H, I]
+        self._super_global_to_local: Optional[torch.Tensor] = None
         self._packed_expert_count = 0
         self._packed_intermediate_size = 0
         self._packed_global_to_local: Optional[torch.Tensor] = None
@@ -112,6 +115,7 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         if layer is not None:
             layer.close()
         self._packed_layer = None
+        self._super_weights = None
 
     def _ensure_runtime_cache(self, device: torch.device) -> None:
         if self._runtime_cache_ready and self._runtime_cache_device == device:
@@ -135,6 +139,10 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         for local, (idx, _) in enumerate(packed_items):
             g2l[idx] = local
         self._packed_global_to_local = g2l.to(device)
+        supers = torch.full((self.num_experts,), -1, dtype=torch.int32)
+        for local, (idx, _) in enumerate(super_items):
+            supers[idx] = local
+        self._super_global_to_local = supers.to(device) if super_items else None
         self._identity_map = self._packed_expert_count == self.num_experts and not super_items
         modules = [m for _, m in packed_items]
         for tag in _TAGS:
@@ -184,9 +192,67 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
             out = module(hidden_states.index_select(0, token_ids)) * flat_route_weights_hidden[rows].unsqueeze(-1)
             final_hidden_states.index_add_(0, token_ids, out.to(hidden_states.dtype))
 
+    def _super_parts(self) -> Optional[List[List[torch.Tensor]]]:
+        """[gate, up, down] weights of every un-quantised expert when all are bias-free SwiGLU MLPs of one shape and 16-bit type."""
+        if str(getattr(self.config, "hidden_act", "silu")).lower() != "silu":
+            return None
+        parts = []
+        for _, module in self._super_expert_items:
+            w = [self._bare_weight(getattr(module, n, None)) for n in ("gate_proj", "up_proj", "down_proj")]
+            if any(p is None for p in w):
+                return None
+            parts.append(w)
+        g = parts[0][0]
+        if g.dtype not in (torch.float16, torch.bfloat16):
+            return None
+        for w in parts:
+            if w[0].shape != g.shape or w[1].shape != g.shape or w[2].shape != g.shape[::-1] or any(p.dtype != g.dtype or p.device != g.device for p in w):
+                return None
+        return parts
+
+    def _stacked_super_weights(self) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
+        """The un-quantised experts' weights as two stacked tensors, whose slices the experts' own parameters become: nothing is held
+        twice, and what is written to a parameter is what the kernels read.  Built again once a parameter lives somewhere else."""
+        parts = self._super_parts()
+        if parts is None:
+            return None
+        inter, hidden = parts[0][0].shape
+        held = self._super_weights
+        if held is not None:
+            gu, dn = held
+            where = [(gu[i, :inter], gu[i, inter:], dn[i]) for i in range(len(parts))]
+            if gu.shape == (len(parts), 2 * inter, hidden) and all(p.data_ptr() == v.data_ptr() and p.is_contiguous() for w, vs in zip(parts, where) for p, v in zip(w, vs)):
+                return held
+        first = parts[0][0]
+        if first.is_cuda and torch.cuda.is_current_stream_capturing():
+            return None                          # the copies would run at the graph's replay
+        with torch.no_grad():
+            gu = torch.empty((len(parts), 2 * inter, hidden), dtype=first.dtype, device=first.device)
+            dn = torch.empty((len(parts), hidden, inter), dtype=first.dtype, device=first.device)
+            for i, w in enumerate(parts):
+                for p, v in zip(w, (gu[i, :inter], gu[i, inter:], dn[i])):
+                    v.copy_(p)
+                    p.data = v
+        self._super_weights = (gu, dn)
+        return self._super_weights
+
+    def _library_super_experts(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
+                               residual: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """residual + the un-quantised experts' weighted outputs by the library (inference; no host sync, so a block with such experts
+        can be captured into a CUDA graph), or None when the modules are of another kind."""
+        if not x.is_cuda or torch.is_grad_enabled() or topk_idx.shape[-1] > 32:
+            return None
+        weights = self._stacked_super_weights()
+        if weights is None or weights[0].dtype != x.dtype or weights[0].device != x.device:
+            return None
+        from bitsmoe_b200.layer import dense_experts
+        return dense_experts(x, topk_idx, topk_w, *weights, global_to_local=self._super_global_to_local, residual=residual)
+
     def prepare_runtime_fastpath(self, warmup: bool = True) -> None:
         device = self._runtime_device()
         self._ensure_runtime_cache(device)
+        if self._super_expert_items and device.type == "cuda":
+            self._stacked_super_weights()
         if warmup:
             self._warmup_runtime_once(device)
 
@@ -242,6 +308,8 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         """SwiGLU MLP ``mlp`` (gate_proj / up_proj / down_proj, bias-free, SiLU) by the library, scaled per token by
         sigmoid(token_gate(x)) when a one-output bias-free Linear is given; None when the module is of another kind."""
         parts = [getattr(mlp, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        if all(isinstance(p, Linear4) for p in parts):
+            return self._library_dense_mlp4(x, parts, token_gate)
         if not (x.is_cuda and all(self._plain_linear(p) for p in parts) and not torch.is_grad_enabled()):
             return None
         if token_gate is not None and not (self._plain_linear(token_gate) and token_gate.weight.shape[0] == 1):
@@ -251,6 +319,30 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         from bitsmoe_b200.layer import dense_mlp
         return dense_mlp(x, parts[0].weight, parts[1].weight, parts[2].weight,
                          None if token_gate is None else token_gate.weight)
+
+    def _library_dense_mlp4(self, x: torch.Tensor, parts, token_gate) -> Optional[torch.Tensor]:
+        """The same for an MLP whose Linears are held in 4 bits (``quantize_shared_experts``)."""
+        if not (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and not torch.is_grad_enabled()) or len({p.group_size for p in parts}) != 1:
+            return None
+        if token_gate is not None and not (self._plain_linear(token_gate) and token_gate.weight.shape[0] == 1):
+            return None
+        from bitsmoe_b200.layer import dense_mlp4
+        return dense_mlp4(x, *(p.packed() for p in parts), group_size=parts[0].group_size,
+                          token_gate_weight=None if token_gate is None else token_gate.weight.detach())
+
+    def quantize_shared_experts(self, group_size: int = 128) -> int:
+        """Holds the shared expert's three Linears in 4 bits from now on (one scale for every ``group_size`` columns of a row); returns
+        how many were replaced.  At decode sizes their 16-bit weights are most of what such a layer reads."""
+        n = 0
+        for name in ("shared_expert", "shared_experts"):
+            mlp = getattr(self, name, None)
+            parts = [getattr(mlp, p, None) for p in ("gate_proj", "up_proj", "down_proj")]
+            if not all(self._plain_linear(p) for p in parts):
+                continue
+            for p, lin in zip(("gate_proj", "up_proj", "down_proj"), parts):
+                setattr(mlp, p, Linear4.from_linear(lin, group_size))
+                n += 1
+        return n
 
     def _bare_weight(self, module) -> Optional[torch.Tensor]:
         """The weight of a bias-free nn.Linear, else None (dict look-ups: this runs per layer and step)."""

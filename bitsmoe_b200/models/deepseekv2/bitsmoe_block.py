@@ -63,10 +63,13 @@ class BitsMoE_DeepSeekSparseMoeBlock(BitsMoE_BaseSparseMoeBlock):
             if residual is None:
                 residual = self.shared_experts(hidden_states).reshape(-1, orig_shape[-1])
         if self._super_expert_items:
-            dense = torch.zeros_like(x)
-            self._run_super_experts(x, dense, idx.reshape(-1).long(), self._get_flat_token_ids(x.shape[0], x.device),
-                                    w.reshape(-1).to(x.dtype))
-            residual = dense if residual is None else residual + dense
+            dense = self._library_super_experts(x, idx, w.to(x.dtype).to(torch.float32), residual)
+            if dense is None:
+                dense = torch.zeros_like(x)
+                self._run_super_experts(x, dense, idx.reshape(-1).long(), self._get_flat_token_ids(x.shape[0], x.device),
+                                        w.reshape(-1).to(x.dtype))
+                dense = dense if residual is None else residual + dense
+            residual = dense
         y = self._fused_forward(x, topk=(idx, w), residual=residual).reshape(*orig_shape)
         if self.training and aux_loss is not None:
             y = AddAuxiliaryLoss.apply(y, aux_loss)

@@ -53,10 +53,13 @@ class BitsMoE_Qwen3MoeSparseMoeBlock(BitsMoE_BaseSparseMoeBlock):
             # dense (unquantised) experts need the selection on the torch side as well
             from bitsmoe_b200.layer import route_topk
             idx, w = route_topk(router_logits, self.top_k, self.norm_topk_prob, x.dtype)
-            dense = torch.zeros_like(x)
-            self._run_super_experts(x, dense, idx.reshape(-1).long(), self._get_flat_token_ids(x.shape[0], x.device),
-                                    w.reshape(-1).to(x.dtype))
-            residual = dense if residual is None else residual + dense
+            dense = self._library_super_experts(x, idx, w, residual)
+            if dense is None:
+                dense = torch.zeros_like(x)
+                self._run_super_experts(x, dense, idx.reshape(-1).long(), self._get_flat_token_ids(x.shape[0], x.device),
+                                        w.reshape(-1).to(x.dtype))
+                dense = dense if residual is None else residual + dense
+            residual = dense
             y = self._fused_forward(x, topk=(idx, w), residual=residual)
         else:
             y = self._fused_forward(x, logits=router_logits, residual=residual)
