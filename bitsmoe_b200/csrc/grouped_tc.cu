@@ -5,8 +5,8 @@
 // (expert, up to 256 of its rows, 256 weight rows): each CTA loads 128 weight rows and half of the item's rows, and the tensor cores
 // read both halves, so that an SM fetches 32 KB per 64 columns of K for 128 x 256 sums (a lone CTA would need 48, which is more than an SM gets
 // from L2 while its tensor core multiplies them).
-//   warp 0      producer: weight rows and rows of x as tiled copies, or rows of x by tile::gather4 (four an instruction), all onto
-//               the even CTA's barrier
+//   warps 0, 3  producers: weight rows as tiled copies; rows of x as tiled copies or by tile::gather4 (four an instruction); all onto
+//               the even CTA's barrier.  A copy costs its thread 50 cycles or more, a stage of nine on one warp more than its products
 //   warp 1      MMA issue, in the even CTA for both: four tcgen05.mma (M = 256, N = the item's rows, K = 16) per stage
 //   warps 4-11  epilogue: tensor memory -> registers (fragments of 16 weight rows x 8 rows) -> y.  stmatrix turns them round in
 //               shared memory, so that a thread stores 16 bytes of a row of y.  With a gated pair the accumulator's lanes alternate between
@@ -34,11 +34,12 @@ constexpr int GC_RING = 6 * 2 * GC_A_BYTES;
 constexpr int gc_smem_bytes(int E) { return GC_RING + GC_EPI_WARPS * GC_TURN_BYTES + 1024 + (3 * E + 1) * 4; }
 
 struct GcParams {
-  CUtensorMap x, x8, w, w32;   // x: 32 rows in order (one row of a gather), or 8; w: 128 weight rows, or 32 (gated pair: 16 and 16)
+  CUtensorMap x, x8;           // 32 rows in order (one row of a gather), 8
+  CUtensorMap w, w32;          // 128 weight rows, or 32 (of a gated pair 16 and 16)
   const int32_t* offsets;
   const int32_t* index;
   void* y;
-  int x_rows, rows, N, E, slices, vec;     // vec: y takes 16-byte stores
+  int x_rows, rows, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
   SlotArgs slots;
 };
 
@@ -66,6 +67,12 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
                    tc::smem_u32(dst)),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_5d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, int w, int v, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(bar)
                : "memory");
 }
 // K-major operand tile of 128-byte rows, 8-row groups 1024 bytes apart, 128-byte swizzle
@@ -192,13 +199,44 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   bool ok = true;
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ producer
+    // ------------------------------------------------------------------ weight rows
+    uint32_t st = 0, ph = 0;
+    int e = 0;
+    for (int item = pair; item < items && ok; item += pairs) {
+      const GcItem it = gc_item(tab, item, e);
+      const uint32_t bytes = 2 * (a_bytes + (it.n() >> 1) * GC_K * 2);      // of both CTAs' slices
+      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
+      for (int k0 = 0; k0 < p.slices; k0 += sub) {
+        if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
+        if (tc::elect_one()) {
+          const int cnt = min(sub, p.slices - k0);
+          const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
+          if (rank == 0) tc::mbar_expect_tx(&full[st], cnt * bytes);
+          for (int j = 0; j < cnt; ++j) {
+            unsigned char* sa = smem + (st * sub + j) * slice;
+            const int k = (k0 + j) * GC_K;
+            if (GLU) {
+              if (quarters == 4 && p.whole) tma_load_5d_pair(sa, &p.w, k, 0, 0, col0 / 16, it.e, bar);
+              else
+                for (int b = 0; b < quarters; ++b) tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 16 * b, 0, it.e, bar);
+            } else if (quarters == 4) {
+              tma_load_3d_pair(sa, &p.w, k, col0, it.e, bar);
+            } else {
+              for (int b = 0; b < quarters; ++b) tma_load_3d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 32 * b, it.e, bar);
+            }
+          }
+        }
+        __syncwarp();
+        if (++st == stages) { st = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ rows of x
     uint32_t st = 0, ph = 0;
     int e = 0;
     for (int item = pair; item < items && ok; item += pairs) {
       const GcItem it = gc_item(tab, item, e);
       const int half = it.n() >> 1, first = it.row0 + static_cast<int>(rank) * half;
-      const uint32_t bytes = 2 * (a_bytes + half * GC_K * 2);      // of both CTAs' slices
       if (GATHER) {
         int id[4];
 #pragma unroll
@@ -211,25 +249,14 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         rows4[lane] = make_int4(id[0], id[1], id[2], id[3]);
         __syncwarp();
       }
-      const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
       for (int k0 = 0; k0 < p.slices; k0 += sub) {
         if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
-        const int cnt = min(sub, p.slices - k0);
-        unsigned char* const s0 = smem + st * (sub * slice);
-        const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
         if (tc::elect_one()) {
-          if (rank == 0) tc::mbar_expect_tx(&full[st], cnt * bytes);
+          const int cnt = min(sub, p.slices - k0);
+          const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
           for (int j = 0; j < cnt; ++j) {
-            unsigned char* sa = s0 + j * slice;
+            unsigned char* const sb = smem + (st * sub + j) * slice + a_bytes;
             const int k = (k0 + j) * GC_K;
-            if (GLU) {
-              for (int b = 0; b < quarters; ++b) tma_load_4d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 16 * b, 0, it.e, bar);
-            } else if (quarters == 4) {
-              tma_load_3d_pair(sa, &p.w, k, col0, it.e, bar);
-            } else {
-              for (int b = 0; b < quarters; ++b) tma_load_3d_pair(sa + b * (GC_A_BYTES / 4), &p.w32, k, col0 + 32 * b, it.e, bar);
-            }
-            unsigned char* const sb = sa + a_bytes;
             if (GATHER) {
 #pragma unroll 4
               for (int r = 0; r < half; r += 4) tma_gather4_pair(sb + r * (GC_K * 2), &p.x, k, rows4[r / 4], bar);
@@ -273,7 +300,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (ok && tc::elect_one()) tc::mma_commit_pair(&acc_full[ab]);
       __syncwarp();
     }
-  } else if (warp == 3) {
+  } else if (warp == 2) {
     // ------------------------------------------------------------------ places of the slots, for whoever sums over a token's experts
     if (p.slots.pos)
       for (int i = blockIdx.x * 32 + lane; i < p.slots.slots; i += gridDim.x * 32) p.slots.pos[i] = slot_place(p.slots, i);
@@ -390,6 +417,12 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
     const cuuint64_t dims[4] = {K, N, 2, E}, strides[3] = {K * 2, N * K * 2, 2 * N * K * 2};
     const cuuint32_t box[4] = {GC_K, 16, 2, 1};
     if (!encode_map16(&p.w32, a.w, 4, dims, strides, box)) return BM_ERR_UNSUPPORTED;
+    if (N % 16 == 0) {
+      // 16 rows, gate or up, block of 16 rows: a CTA's 128 operand rows in one copy
+      const cuuint64_t dims5[5] = {K, 16, 2, N / 16, E}, strides5[4] = {K * 2, N * K * 2, 16 * K * 2, 2 * N * K * 2};
+      const cuuint32_t box5[5] = {GC_K, 16, 2, 4, 1};
+      p.whole = encode_map16(&p.w, a.w, 5, dims5, strides5, box5);
+    }
   } else {
     const cuuint64_t dims[3] = {K, N, E}, strides[2] = {K * 2, N * K * 2};
     const cuuint32_t box[3] = {GC_K, 128, 1}, box32[3] = {GC_K, 32, 1};

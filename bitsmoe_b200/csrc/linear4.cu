@@ -190,21 +190,19 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   // ---- sums of the warps (and CTAs) that share the rows, then out
   auto finish_unit = [&](int rb) {
     const int ra = (rb * rws + rw) * per + g, rc = ra + 8;
-    auto finish = [&](int row, int n, float v) { linear4_finish<XD>(a, n0 + n, row, v); };
     if (a.kwarps == 1 && a.splits == 1) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = 8 * b + 2 * t + i;
-          if (n >= nn) continue;
-          if (a.glu) {
-            if (ra < a.N) finish(ra, n, silu_mul(acc[b][i], acc[b][2 + i]));
-          } else {
-            if (ra < a.N) finish(ra, n, acc[b][i]);
-            if (rc < a.N) finish(rc, n, acc[b][2 + i]);
-          }
+      for (int b = 0; b < NB; ++b) {
+        auto token = [&](int row, int i) { return 8 * b + 2 * t + i < nn && row < a.N ? n0 + 8 * b + 2 * t + i : -1; };
+        if (a.glu) {
+          const float z[2] = {silu_mul(acc[b][0], acc[b][2]), silu_mul(acc[b][1], acc[b][3])};
+          linear4_finish<XD>(a, ra, z, [&](int i) { return token(ra, i); });
+        } else {
+          const float lo[2] = {acc[b][0], acc[b][1]}, hi[2] = {acc[b][2], acc[b][3]};
+          linear4_finish<XD>(a, ra, lo, [&](int i) { return token(ra, i); });
+          linear4_finish<XD>(a, rc, hi, [&](int i) { return token(rc, i); });
         }
+      }
       return;
     }
     constexpr int COLS = 8 * NB, PART = 16 * COLS;       // floats of one warp's part: [row][token]
@@ -232,7 +230,8 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
             v += part[row * COLS];
             if (a.glu) u += part[(row + 8) * COLS];
           }
-        finish(out_row, n, a.glu ? silu_mul(v, u) : v);
+        const float out[1] = {a.glu ? silu_mul(v, u) : v};
+        linear4_finish<XD>(a, out_row, out, [&](int) { return n0 + n; });
       }
     }
     if (a.splits == 1) __syncthreads();                  // the parts may be overwritten

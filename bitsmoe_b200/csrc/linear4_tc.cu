@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
     uint32_t acc = 0;                          // groups so far: buffer acc % LT_ACC
-    const int run = min(p.per_group, LT_K / 16);
+    const bool two = p.per_group == 2;
     int s = 0, bs = 0, b_ph = 0;
     for (int i = 0; i < mine && ok; ++i) {
       int row0, tok0, n;
@@ -147,29 +147,34 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       for (int k = 0; k < slices && ok; ++k, ++s) {
         const int st = s % LT_AS;
         if (!(ok = tc::mbar_wait(&b_full[bs], b_ph) && tc::mbar_wait(&a_ready[st], (s / LT_AS) & 1))) break;
+        tc::fence_after_sync();
         const uint64_t ad = lt_desc(tc::smem_u32(smem + st * LT_A_BYTES)), bd = lt_desc(tc::smem_u32(b_ring + bs * b_bytes));
         // the slice's products of one group at a time: four, or two and two
-        for (int kk = 0; kk < LT_K / 16; kk += run) {
-          const uint32_t buf = acc % LT_ACC;
-          if (in_group == 0 && acc >= LT_ACC && !(ok = tc::mbar_wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
-          tc::fence_after_sync();
-          const bool last = in_group + run == p.per_group || (k + 1 == slices && kk + run == LT_K / 16);
+        const bool end = k + 1 == slices;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !two) break;
+          const uint32_t buf = acc % LT_ACC, d = tmem_base + buf * LT_TOK;
+          if (in_group == 0) {
+            if (acc >= LT_ACC && !(ok = tc::mbar_wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
+            tc::fence_after_sync();
+          }
+          const bool last = two || in_group + 4 == p.per_group || end;
           if (tc::elect_one()) {
-            const uint32_t d = tmem_base + buf * LT_TOK;
-            tc::mma_f16(d, ad + 2 * kk, bd + 2 * kk, idesc, in_group > 0 ? 1u : 0u);
-            tc::mma_f16(d, ad + 2 * kk + 2, bd + 2 * kk + 2, idesc, 1u);
-            if (run == 4) {
+            tc::mma_f16(d, ad + 4 * h, bd + 4 * h, idesc, in_group > 0 ? 1u : 0u);
+            tc::mma_f16(d, ad + 4 * h + 2, bd + 4 * h + 2, idesc, 1u);
+            if (!two) {
               tc::mma_f16(d, ad + 4, bd + 4, idesc, 1u);
               tc::mma_f16(d, ad + 6, bd + 6, idesc, 1u);
             }
             if (last) tc::mma_commit(&acc_full[buf]);
-            if (kk + run == LT_K / 16) {
+            if (h == 1 || !two) {
               tc::mma_commit(&a_empty[st]);
               tc::mma_commit(&b_empty[bs]);
             }
           }
           __syncwarp();
-          in_group = last ? 0 : in_group + run;
+          in_group = last ? 0 : in_group + 4;
           acc += last;
         }
         if (++bs == b_stages) { bs = 0; b_ph ^= 1; }
@@ -287,16 +292,21 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
         const int c0 = 16 * (half + 2 * b);
         if (c0 >= n) break;
         if (GLU) {
+          float z[8];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float other = __shfl_xor_sync(0xffffffffu, up ? sum[b][j] : sum[b][j + 1], 16);
-            const int tok = tok0 + c0 + j + up;
-            if (tok < p.a.T && row < p.a.N) linear4_finish<XD>(p.a, tok, row, up ? silu_mul(other, sum[b][j + 1]) : silu_mul(sum[b][j], other));
+            z[j / 2] = up ? silu_mul(other, sum[b][j + 1]) : silu_mul(sum[b][j], other);
           }
-        } else if (row < p.a.N) {
+          linear4_finish<XD>(p.a, row, z, [&](int j) { return tok0 + c0 + 2 * j + up < p.a.T && row < p.a.N ? tok0 + c0 + 2 * j + up : -1; });
+        } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (tok0 + c0 + j < p.a.T) linear4_finish<XD>(p.a, tok0 + c0 + j, row, sum[b][j]);
+          for (int h = 0; h < 2; ++h) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = sum[b][8 * h + j];
+            linear4_finish<XD>(p.a, row, v, [&](int j) { return tok0 + c0 + 8 * h + j < p.a.T && row < p.a.N ? tok0 + c0 + 8 * h + j : -1; });
+          }
         }
       }
     }
