@@ -87,8 +87,10 @@ __global__ void __launch_bounds__(256) row_gate_kernel(const void* __restrict__ 
                                                        int beside) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = (blockIdx.x * (blockDim.x >> 5) + warp) * RG_TOKENS;
-  grid_launch_dependents();
-  if (!beside) grid_wait();
+  // 0: waits for the launches before it; 1: runs beside them; 2: waits, and lets the next launch run beside itself
+  if (beside != 2) grid_launch_dependents();
+  if (beside != 1) grid_wait();
+  if (beside == 2) grid_launch_dependents();
   auto weight = [&](uint32_t v) {
     const float2 f = row_gate_pair<WD>(v);
     return WD == BM_F16 ? f : __half22float2(__floats2half2_rn(f.x, f.y));
@@ -134,16 +136,17 @@ __global__ void __launch_bounds__(256) row_gate_kernel(const void* __restrict__ 
       if (lane == 0) gate[t] = 1.f / (1.f + __expf(-acc));
     }
   }
-  if (beside) grid_wait();
+  if (beside == 1) grid_wait();
 }
 
-int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st) {
+// `lead`: the next launch on the stream is an AFTER_BESIDE one that reads what was there before this launch.
+int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st, bool lead) {
   const int per = 8 * RG_TOKENS;
   const bool wh = w_dtype == BM_F16;
   auto* kernel = x_dtype == BM_F32 ? (wh ? row_gate_kernel<BM_F32, BM_F16> : row_gate_kernel<BM_F32, BM_BF16>)
                  : x_dtype == BM_F16 ? (wh ? row_gate_kernel<BM_F16, BM_F16> : row_gate_kernel<BM_F16, BM_BF16>)
                                      : (wh ? row_gate_kernel<BM_BF16, BM_F16> : row_gate_kernel<BM_BF16, BM_BF16>);
-  BM_CUDA(launch_after(after, 1, kernel, dim3((T + per - 1) / per), 256, 0, st, x, w, T, H, gate, after == AFTER_BESIDE));
+  BM_CUDA(launch_after(after, 1, kernel, dim3((T + per - 1) / per), 256, 0, st, x, w, T, H, gate, after == AFTER_BESIDE ? 1 : lead ? 2 : 0));
   BM_LAUNCH_CHECK("row_gate_kernel");
   return BM_OK;
 }

@@ -18,11 +18,11 @@ namespace cg = cooperative_groups;
 
 namespace bm {
 
-int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st);
+int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st, bool lead);
 
 constexpr int L4_THREADS = 256, L4_WARPS = 8, L4_CHUNK = 128;
-__host__ __device__ constexpr int l4_batch(int nt) { return nt <= 8 ? 2 : 4; }      // chunks in flight a warp and buffer
-__host__ __device__ constexpr int l4_ctas(int nt) { return nt <= 8 ? 3 : 2; }       // CTAs an SM
+__host__ __device__ constexpr int l4_batch(int nt) { return 4; }      // chunks in flight a warp and buffer
+__host__ __device__ constexpr int l4_ctas(int nt) { return 2; }       // CTAs an SM
 constexpr size_t L4_SMEM = 110 * 1024;          // two CTAs an SM
 
 template <int XD>
@@ -46,6 +46,13 @@ template <int NT>
 __device__ __forceinline__ int l4_piece(int place, int n) {
   const int t = place & 3, sw = NT >= 8 ? 2 * t : 0;
   return (place * NT + (n ^ sw)) * 16;
+}
+
+// Weights are read once: past the first-level cache.
+__device__ __forceinline__ uint4 l4_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
 template <int NT, int XD, int WPL>
@@ -76,25 +83,36 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
     if (f_rb >= a.row_blocks) return;
     // codes behind the matrix meet zeros of x, chunks behind the warp's are not multiplied: any word of the row will do there
     const int first = (c_first + f_c) * (L4_CHUNK / 8) + t * WPL, last = a.words - WPL;
+    auto load = [&](int u, int j, const uint32_t* sa_, const uint32_t* sc_) {
 #pragma unroll
-    for (int u = 0; u < L4_BATCH; ++u)
-#pragma unroll
-      for (int j = 0; j < GPC; ++j) {
-        const int at = min(first + u * (L4_CHUNK / 8) + j * 4 * WPL, last);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t* src = (r ? pc : pa) + at;
-          if (WPL == 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-            wd[r][u][0] = v.x; wd[r][u][1] = v.y; wd[r][u][2] = v.z; wd[r][u][3] = v.w;
-          } else if (WPL == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-            wd[r][u][2 * j] = v.x; wd[r][u][2 * j + 1] = v.y;
-          } else {
-            wd[r][u][j] = __ldg(src);
-          }
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t* src = r ? sc_ : sa_;
+        if (WPL == 4) {
+          const uint4 v = l4_stream(reinterpret_cast<const uint4*>(src));
+          wd[r][u][0] = v.x; wd[r][u][1] = v.y; wd[r][u][2] = v.z; wd[r][u][3] = v.w;
+        } else if (WPL == 2) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+          wd[r][u][2 * j] = v.x; wd[r][u][2 * j + 1] = v.y;
+        } else {
+          wd[r][u][j] = __ldg(src);
         }
       }
+    };
+    if (first + (L4_BATCH * L4_CHUNK / 8 - 4 * WPL) <= last) {       // the whole batch lies inside the row: one address a row
+      const uint32_t *qa = pa + first, *qc = pc + first;
+#pragma unroll
+      for (int u = 0; u < L4_BATCH; ++u)
+#pragma unroll
+        for (int j = 0; j < GPC; ++j) load(u, j, qa + u * (L4_CHUNK / 8) + j * 4 * WPL, qc + u * (L4_CHUNK / 8) + j * 4 * WPL);
+    } else {
+#pragma unroll
+      for (int u = 0; u < L4_BATCH; ++u)
+#pragma unroll
+        for (int j = 0; j < GPC; ++j) {
+          const int at = min(first + u * (L4_CHUNK / 8) + j * 4 * WPL, last);
+          load(u, j, pa + at, pc + at);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < SPR; ++i) {
       const int grp = (c_first + f_c) * GPC + 4 * i + t;
@@ -112,7 +130,7 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   uint32_t w[2][2][L4_BATCH][4];           // [buffer][row][chunk][word]
   float sv[2][2][SPR];                     // lane t: scale of group 4 i + t of the batch
   grid_launch_dependents();
-  if (!a.early) grid_wait();
+  if (!a.early && !a.beside) grid_wait();
   fetch(w[0], sv[0]);
   if (a.early) grid_wait();
   // ---- x of this CTA's columns, in the order of the products
@@ -254,6 +272,7 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   };
   while (step(w[0], sv[0], w[1], sv[1]) && step(w[1], sv[1], w[0], sv[0])) {
   }
+  if (a.beside) grid_wait();
 }
 
 constexpr int L4_TOKENS = 16;        // above, the tensor core's kernel
@@ -369,11 +388,11 @@ extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* g
   const int ldz = static_cast<int>(align_up(intermediate, 8));
   void* z = workspace;
   float* gate = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align_up(static_cast<size_t>(T) * ldz * 2, 256));
-  if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_READS, st))) return rc;
+  if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_READS, st, true))) return rc;
   Linear4Args a{};
   a.p[0] = gate_payload; a.p[1] = up_payload;
   a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
-  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1;
+  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1; a.beside = token_gate_w != nullptr;
   if ((rc = linear4(a, dtype, group, AFTER_READS, st))) return rc;
   Linear4Args d{};
   d.p[0] = down_payload; d.s[0] = reinterpret_cast<const __half*>(down_scale);

@@ -13,7 +13,8 @@ struct Linear4Args {
   const float* row_gate;       // factor per token, or null
   void* y;                     // [T, ldy]
   int T, K, N, ldx, ldy, words, groups;
-  int glu, vec_x, kwarps, splits, row_blocks, early;     // early: the launch before wrote none of the weights
+  int glu, vec_x, kwarps, splits, row_blocks;
+  int early, beside;           // the launch before wrote none of the weights; nothing that this one reads (an AFTER_BESIDE launch behind a `lead` one)
 };
 
 // Eight codes -> four pairs (code i, code i + 4), i = 0 .. 3, as exact numbers -8 .. 7 of the type.

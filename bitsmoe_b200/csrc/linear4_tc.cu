@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   tc::fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   grid_launch_dependents();
-  grid_wait();
+  if (!p.a.beside) grid_wait();
   // tiles of this CTA (neighbours share weight rows), and its slices of their columns: all, or a share that starts with a group
   const int rank = blockIdx.x % p.splits, first = blockIdx.x / p.splits, grid = gridDim.x / p.splits, tiles = p.row_tiles * p.tok_tiles;
   const int mine = tiles > first ? (tiles - first + grid - 1) / grid : 0;
@@ -316,6 +316,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       tc::cluster_arrive();
       tc::cluster_wait();
     }
+  if (p.a.beside) grid_wait();
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 2) tc::tmem_dealloc(tmem_base, 512);

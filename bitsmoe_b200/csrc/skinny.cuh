@@ -60,7 +60,7 @@ bool skinny_many_waves(int row_tiles, int splits, int T);
 int skinny_splits(int rows, int K);
 
 // gate[t] = sigmoid(x[t] . w) (dense.cu)
-int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st);
+int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, int T, int H, float* gate, LaunchAfter after, cudaStream_t st, bool lead = false);
 
 bool route_small_fits(int T, int E, int k);
 int launch_route_small(const RouteSmallArgs& a, cudaStream_t st);
