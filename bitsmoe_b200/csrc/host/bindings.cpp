@@ -309,6 +309,10 @@ int half_code(const at::Tensor& t, const char* msg) {
   return dtype_code(t.scalar_type());
 }
 void require_int32_range(int64_t v, const char* msg) { require(v <= 0x7fffffff, msg); }
+bool overlap(const at::Tensor& a, const at::Tensor& b) {      // of contiguous tensors
+  const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
+  return a.numel() && b.numel() && pa < pb + b.nbytes() && pb < pa + a.nbytes();
+}
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, like.options().dtype(at::kByte));
 }
@@ -332,6 +336,8 @@ PyObject* grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(!out.defined() || (out.device() == x.device() && out.scalar_type() == x.scalar_type() && out.is_contiguous() && out.dim() == 2 &&
                                out.size(0) == rows && out.size(1) == w.size(1)),
             "grouped_linear: out must be contiguous [rows, N] of x's type and device");
+    for (const at::Tensor* t : {&x, &w})
+      require(!out.defined() || !overlap(out, *t), "grouped_linear: out overlaps an input");
     const c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor y = out.defined() ? out : at::empty({rows, w.size(1)}, x.options());
     const size_t need = tok.defined() ? bm_grouped_linear_workspace_bytes(static_cast<int32_t>(x.size(1)), static_cast<int32_t>(w.size(0)), static_cast<int32_t>(rows)) : 0;

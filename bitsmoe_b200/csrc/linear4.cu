@@ -23,7 +23,7 @@ int launch_row_gate(const void* x, int x_dtype, const uint16_t* w, int w_dtype, 
 constexpr int L4_THREADS = 256, L4_WARPS = 8, L4_CHUNK = 128;
 __host__ __device__ constexpr int l4_batch(int nt) { return 4; }      // chunks in flight a warp and buffer
 __host__ __device__ constexpr int l4_ctas(int nt) { return 2; }       // CTAs an SM
-constexpr size_t L4_SMEM = 110 * 1024;          // two CTAs an SM
+constexpr size_t L4_SMEM = 110 * 1024, L4_SMEM_MOST = 220 * 1024;          // two CTAs an SM, one
 
 template <int XD>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
@@ -275,7 +275,9 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   if (a.beside) grid_wait();
 }
 
-constexpr int L4_TOKENS = 16;        // above, the tensor core's kernel
+// Tokens up to which the weights are streamed; above, the tensor core's kernel.  us, bf16, groups of 128: K 2048, N 4096: 16 tokens 8.7 / 13.6, 32 tokens
+// 24 / 14; N 100003: 16 tokens 44 / 96, 32 tokens 159 / 97.
+constexpr int L4_TOKENS = 16;
 
 static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
   const int chunks = (K + L4_CHUNK - 1) / L4_CHUNK, cols = nt < 8 ? 8 : nt;
@@ -288,7 +290,7 @@ static int l4_launch_one(const Linear4Args& a, dim3 grid, size_t smem, LaunchAft
   int dev = -1;
   BM_CUDA(cudaGetDevice(&dev));
   if (!once.is_done(dev)) {
-    BM_CUDA(cudaFuncSetAttribute(linear4_kernel<NT, XD, WPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    BM_CUDA(cudaFuncSetAttribute(linear4_kernel<NT, XD, WPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L4_SMEM_MOST)));
     once.mark(dev);
   }
   BM_CUDA(launch_after(after, a.splits, linear4_kernel<NT, XD, WPL>, grid, L4_THREADS, smem, st, a));
@@ -310,21 +312,33 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
   a.words = (a.K + 31) / 32 * 4;
   a.groups = (a.K + group - 1) / group;
   a.vec_x = aligned16(a.x) && a.ldx % 8 == 0;
-  if (a.T > L4_TOKENS) {
+  static PerDeviceOnce once;
+  static int sm_counts[MAX_DEVICES];
+  int dev = -1;
+  BM_CUDA(cudaGetDevice(&dev));
+  BM_REQUIRE(dev >= 0 && dev < MAX_DEVICES, BM_ERR_UNSUPPORTED, "linear4: device ordinal %d out of range", dev);
+  if (!once.is_done(dev)) {
+    BM_CUDA(cudaDeviceGetAttribute(&sm_counts[dev], cudaDevAttrMultiProcessorCount, dev));
+    once.mark(dev);
+  }
+  const int sms = sm_counts[dev];
+  const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK, units = (a.N + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
+  int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32;
+  a.kwarps = 1; a.splits = 1;
+  while (nt > 8 && l4_smem_bytes(nt, a.K, 8, true) > L4_SMEM_MOST) nt /= 2;
+  while (a.splits < 8 && l4_smem_bytes(nt, a.K, a.splits, true) > L4_SMEM) a.splits *= 2;
+  const bool fits = l4_smem_bytes(nt, a.K, a.splits, true) <= L4_SMEM_MOST && (a.T + nt - 1) / nt <= 65535;
+  if (a.T > L4_TOKENS || !fits) {
     const int rc = launch_linear4_tc(a, x_dtype, group, after, st);
     if (rc != BM_ERR_UNSUPPORTED) return rc;
   }
-  const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK, units = (a.N + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
-  int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32;
-  // warps of a CTA, then CTAs of a cluster, share a row's columns until every SM has work
-  a.kwarps = 1; a.splits = 1;
-  while (nt > 8 && l4_smem_bytes(nt, a.K, 8, true) > 200 * 1024) nt /= 2;
-  while (a.splits < 8 && l4_smem_bytes(nt, a.K, a.splits, true) > L4_SMEM) a.splits *= 2;
-  while (a.kwarps < 8 && 2 * a.kwarps * a.splits <= chunks && units * a.kwarps < 148 * 16) a.kwarps *= 2;
-  BM_REQUIRE(l4_smem_bytes(nt, a.K, a.splits, true) <= 220 * 1024, BM_ERR_UNSUPPORTED, "linear4: %d columns are too many", a.K);
+  BM_REQUIRE(fits, BM_ERR_UNSUPPORTED, "linear4: %d rows of %d columns that do not start on 16-byte boundaries", a.T, a.K);
+  // warps of a CTA share a row's columns until every SM has work (sharing costs a barrier and a pass over the parts per row block: 100003 rows 36 us with
+  // none, 38, 44 and 59 with two, four and eight warps)
+  while (a.kwarps < 8 && 2 * a.kwarps * a.splits <= chunks && units * a.kwarps < sms * 16) a.kwarps *= 2;
   const int rws = L4_WARPS / a.kwarps;
   a.row_blocks = (units + rws - 1) / rws;
-  const int most = 148 * l4_ctas(nt) / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
+  const int most = sms * l4_ctas(nt) / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
   const dim3 g(grid, (a.T + nt - 1) / nt);
   const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
   switch (nt) {

@@ -226,7 +226,7 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         first = parts[0][0]
         if first.is_cuda and torch.cuda.is_current_stream_capturing():
             return None                          # the copies would run at the graph's replay
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():        # the parameters stay ordinary tensors, whatever mode the first call is in
             gu = torch.empty((len(parts), 2 * inter, hidden), dtype=first.dtype, device=first.device)
             dn = torch.empty((len(parts), hidden, inter), dtype=first.dtype, device=first.device)
             for i, w in enumerate(parts):

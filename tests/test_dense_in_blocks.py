@@ -110,6 +110,22 @@ def test_block_with_super_experts_can_be_captured():
 
 
 @gpu
+def test_first_call_in_inference_mode_leaves_ordinary_parameters():
+    cfg, blk = _qwen_block([2, 5])
+    x = torch.randn(1, 7, cfg.hidden, generator=torch.Generator().manual_seed(4)).to(DEV).half()
+    with torch.inference_mode():
+        first, _ = blk(x)
+    assert blk._super_weights is not None
+    w = blk.experts[5].gate_proj.weight
+    assert not w.is_inference() and not blk._super_weights[0].is_inference()
+    blk.experts[5](x[0]).float().sum().backward()                       # the modules still train
+    assert w.grad is not None and w.grad.shape == w.shape
+    with torch.no_grad():
+        w.mul_(0.5)
+        helpers.assert_close(blk(x)[0], _by_modules(blk, x)[0], what="after inference mode")
+
+
+@gpu
 def test_modules_of_another_kind_keep_their_own_forward():
     cfg, blk = _qwen_block([2])
     x = torch.randn(1, 9, cfg.hidden, generator=torch.Generator().manual_seed(3)).to(DEV).half()

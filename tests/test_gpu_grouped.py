@@ -39,6 +39,8 @@ SIZES = {
     "every size at a tile's edge": [1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 255, 256, 257, 2],
     "one long among short": [3, 1, 700, 2, 0, 1],
     "many groups": [(7 * i) % 5 for i in range(200)],
+    "more groups than the tensor-core kernel's table holds": [(7 * i) % 3 for i in range(1100)],
+    "rows enough to be brought into order first": [150, 0, 90, 131],
 }
 SHAPES = [(64, 128), (2048, 256), (768, 2048), (200, 136), (8, 1), (1000, 999), (72, 257)]     # (K, N): rows of 16-byte multiples
 ODD = [(67, 33), (1, 1), (129, 70), (1001, 48)]
@@ -271,6 +273,8 @@ def test_refusals():
              lambda: grouped_linear(x, w, off, out=h(5, 32)), lambda: grouped_linear(x, w, off, out=h(6, 32).bfloat16()),
              lambda: grouped_linear(x, w, off, out=h(32, 6).t()), lambda: grouped_linear(x.clone().requires_grad_(), w, off),
              lambda: grouped_linear(x, w.clone().requires_grad_(), off), lambda: grouped_linear(x.reshape(2, 3, 64), w, off)]
+    buf = h(6 * 64 + 8)
+    wrong.append(lambda: grouped_linear(buf[:384].view(6, 64), h(1, 64, 64), i32(2), out=buf[8:392].view(6, 64)))       # in place
     idx, tw, gu, dn = i32(6, 2), h(6, 2, dtype=torch.float32), h(3, 64, 64), h(3, 64, 32)
     good = dict(x=x, topk_idx=idx, topk_w=tw, w_gate_up=gu, w_down=dn)
     bad = [dict(x=x.float()), dict(x=h(5, 64)), dict(topk_idx=idx.float()), dict(topk_idx=idx.cpu()), dict(topk_w=h(6, 3)), dict(topk_w=idx),

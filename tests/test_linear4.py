@@ -101,7 +101,7 @@ def test_tokens(tokens, group, dtype):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,k,group", [(1, 1, 128), (5, 7, 32), (16, 32, 32), (17, 100, 64), (999, 1000, 128), (64, 129, 128), (48, 127, 128), (2048, 4096, 64),
-                                       (31, 8200, 32), (4096, 257, 64), (130, 33, 64), (40000, 64, 32), (24, 20000, 128), (7, 65000, 128)])
+                                       (31, 8200, 32), (4096, 257, 64), (130, 33, 64), (40000, 64, 32), (24, 20000, 128), (7, 65000, 128), (40, 120000, 64)])
 @pytest.mark.parametrize("tokens", [1, 5, 40, 200])
 def test_shapes(tokens, n, k, group, dtype):
     gen = torch.Generator().manual_seed(n + k)
