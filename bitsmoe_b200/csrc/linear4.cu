@@ -333,12 +333,18 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
     if (rc != BM_ERR_UNSUPPORTED) return rc;
   }
   BM_REQUIRE(fits, BM_ERR_UNSUPPORTED, "linear4: %d rows of %d columns that do not start on 16-byte boundaries", a.T, a.K);
-  // warps of a CTA share a row's columns until every SM has work (sharing costs a barrier and a pass over the parts per row block: 100003 rows 36 us with
-  // none, 38, 44 and 59 with two, four and eight warps)
-  while (a.kwarps < 8 && 2 * a.kwarps * a.splits <= chunks && units * a.kwarps < sms * 16) a.kwarps *= 2;
+  // Warps of a CTA that share a row's columns: what leaves the fewest chunks one after the other.  A barrier and the pass over the parts cost a chunk and
+  // a half per row block, a cluster's barriers three: 100003 rows of 2048 columns with one, two, four and eight warps 36, 38, 44 and 59 us.
+  const int most = sms * l4_ctas(nt) / a.splits, per_split = (chunks + a.splits - 1) / a.splits;
+  double best = 1e30;
+  for (int kw = 1; kw <= 8 && (kw == 1 || kw * a.splits <= chunks); kw *= 2) {
+    const int blocks = (units + L4_WARPS / kw - 1) / (L4_WARPS / kw), rounds = (blocks + most - 1) / most;
+    const double cost = rounds * ((per_split + kw - 1) / kw + (kw > 1 ? 1.5 : 0.3) + (a.splits > 1 ? 3.0 : 0.0));
+    if (cost < best) { best = cost; a.kwarps = kw; }
+  }
   const int rws = L4_WARPS / a.kwarps;
   a.row_blocks = (units + rws - 1) / rws;
-  const int most = sms * l4_ctas(nt) / a.splits, grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
+  const int grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
   const dim3 g(grid, (a.T + nt - 1) / nt);
   const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
   switch (nt) {
