@@ -13,6 +13,10 @@
 //               16 gate rows and the 16 up rows that belong to them, so that a thread holds both sums of an output.
 // The accumulator alternates between two halves of tensor memory.  Items are handed out round robin; which expert an item belongs
 // to every CTA works out from the offsets, so that the host never reads them.  Waits are bounded.
+//
+// Measured (bf16, K 2048, N 1536): 128 groups in order of 1 row 121 us (HBM floor 123), 128 rows 151, 512 rows 315 (1.3 PFLOP/s); one group of 65536 rows 290
+// (1.42 PFLOP/s, what the library product reaches under the power limit).  Few rows are bound by HBM, many by the tensor pipe at its
+// sustained clock, one to eight groups of one row (11 to 13 us) by start, first data and end of the launch.
 #include <cuda.h>
 
 #include <cstring>

@@ -8,6 +8,9 @@
 // 16-bit numbers -8 .. 7 of x's type by mask and subtraction of a constant; products of a group are summed in fp32 by the tensor
 // core and multiplied by the group's scale in fp32, so nothing but the output is rounded.  Few rows: the eight warps of a CTA and the
 // CTAs of a cluster share a row's columns and meet in shared memory, in a fixed order.
+//
+// Measured (groups of 128): K 2048, N 100003, 4 tokens 35.6 us in bf16 and 32 in fp16 (3.0 and 3.3 TB/s; floor 16.3): 40 instructions for 512 codes, with
+// four warps a scheduler.  K 2048, N 4096, one token 4.5 us inside a graph, 8192 x 8192 at 1 / 8 / 16 tokens 15 / 20 / 29 (floor 5.3).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -13,6 +13,9 @@
 // Where there are few tiles, clusters of CTAs share a tile's columns and add their sums up in the first one's shared memory, in order.
 // With a gated pair the rows alternate between 16 gate rows and the 16 up rows that belong to them; lanes l and l + 16 exchange every
 // other token's sums at the end.  Waits are bounded.
+//
+// Measured (bf16, groups of 128): 4096 x 4096 at 64 / 256 / 1024 tokens 19 / 27 / 76 us (0.11 / 0.31 / 0.45 PFLOP/s).  A slice of 64 columns costs 0.45 us of waits, four
+// products and commits whatever the tile's width, a launch 8 to 10 us of start, first data, exchange and end.
 #include <cuda.h>
 
 #include <cstring>
