@@ -246,9 +246,8 @@ struct DenseExpertsWs {
     pos = take(A * 4);
     off = take(static_cast<size_t>(E + 1) * 4);
     route = take(bm_route_build_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(k), static_cast<int32_t>(E)));
-    xs = take(A * H * 2);
     z = take(A * I * 2);
-    d = take(A * H * 4);
+    d = xs = take(A * H * 4);      // rows of x in expert order are read before the down products are written
     total = at;
   }
 };
@@ -306,7 +305,7 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
   int32_t *tok = reinterpret_cast<int32_t*>(ws + at.tok), *off = reinterpret_cast<int32_t*>(ws + at.off);
   const int A = T * k;
   int rc = bm_route_build(topk_idx, topk_w, global_to_local, num_routed, T, k, num_local, 128, tok, off, reinterpret_cast<float*>(ws + at.rw), nullptr,
-                          nullptr, ws + at.route, at.xs - at.route, stream);
+                          nullptr, ws + at.route, at.z - at.route, stream);
   if (rc) return rc;
   GroupedArgs g{};
   g.x = x; g.w = w_gate_up; g.offsets = off; g.index = tok; g.y = ws + at.z;
@@ -318,7 +317,7 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
   g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
   g.x_rows = A; g.K = intermediate; g.N = hidden; g.glu = 0;
   int32_t* pos = reinterpret_cast<int32_t*>(ws + at.pos);
-  g.slots = SlotArgs{topk_idx, global_to_local, tok, off, pos, A, k, num_local, num_routed};
+  g.slots = SlotArgs{topk_idx, global_to_local, tok, off, pos, A, k, num_local, num_routed, g.expected < A / 4};
   if ((rc = launch_grouped(g, st))) return rc;
   CombineArgs c{};
   c.d = reinterpret_cast<const float*>(ws + at.d);

@@ -10,6 +10,7 @@ struct SlotArgs {
   const int32_t *topk_idx, *map, *token_indices, *offsets;
   int32_t* pos;                // [T * k]; null: nothing to do
   int slots, k, E, num_routed;
+  int sparse;                  // most slots name experts that are not held here
 };
 
 // y[i][n] = sum_k x[row(i)][k] * w[e][n][k] for offsets[e] <= i < offsets[e + 1], row(i) = index[i] (i itself when null).

@@ -113,6 +113,14 @@ __device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int& e) 
   return it;
 }
 
+// Places of the slots by warp `w` of those that take part: one a CTA, or where few of the slots are held here, and the products therefore short, the
+// epilogue warps before their first item too.
+__device__ __forceinline__ void gc_places(const SlotArgs& a, int w, int lane) {
+  const int warps = a.sparse ? 1 + GC_EPI_WARPS : 1;
+  if (a.pos && w < warps)
+    for (int i = (blockIdx.x * warps + w) * 32 + lane; i < a.slots; i += gridDim.x * warps * 32) a.pos[i] = slot_place(a, i);
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t gc_pack(float a, float b) {
   if (BF16) {
@@ -153,7 +161,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     tc::mbar_init_fence();
   }
   if (threadIdx.x == 32) {
-    for (const CUtensorMap* m : {&p.x, &p.x8, &p.w, &p.w32}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+    auto prefetch = [](const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory"); };
+    prefetch(&p.x);
+    prefetch(&p.w32);
+    if (!GATHER) prefetch(&p.x8);
+    if (!GLU || p.whole) prefetch(&p.w);
   }
   __syncthreads();
   tc::cluster_arrive();
@@ -306,11 +318,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ places of the slots, for whoever sums over a token's experts
-    if (p.slots.pos)
-      for (int i = blockIdx.x * 32 + lane; i < p.slots.slots; i += gridDim.x * 32) p.slots.pos[i] = slot_place(p.slots, i);
+    gc_places(p.slots, 0, lane);
   } else if (warp >= GC_EPI0) {
     // ------------------------------------------------------------------ epilogue: lane quarter q, every other block of 32 rows
     const int q = warp & 3, half = (warp - GC_EPI0) >> 2;
+    gc_places(p.slots, warp - GC_EPI0 + 1, lane);
     constexpr int WIDE = GLU ? 16 : 32, PITCH = GLU ? 48 : GC_TURN_PITCH, PIECES = WIDE / 8;      // columns of y a warp has, bytes between rows, 16-byte pieces
     unsigned char* const mine = turn + (warp - GC_EPI0) * GC_TURN_BYTES;
     uint32_t ti = 0;

@@ -269,7 +269,8 @@ BM_API int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_
  * host round trips):  y[t] = residual[t] + sum over slots s of topk_w[t, s] * w_down[e] . (silu(gate_e . x[t]) * (up_e . x[t])),
  * e = global_to_local[topk_idx[t, s]] (the id itself when the map is NULL, and then num_routed must equal num_local); slots whose id
  * is not held here add nothing.  w_gate_up [num_local, 2 * intermediate, hidden], gate rows before up rows; w_down [num_local, hidden,
- * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits. */
+ * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits.  The workspace holds
+ * T * k rows of 4 * hidden + 2 * intermediate bytes and the routing lists, whatever share of the slots is held here. */
 BM_API size_t bm_dense_experts_workspace_bytes(int32_t T, int32_t k, int32_t num_local, int32_t hidden, int32_t intermediate);
 BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* topk_idx, const float* topk_w, const int32_t* global_to_local,
                                     int32_t num_routed, int32_t T, int32_t k, int32_t num_local, const void* w_gate_up,

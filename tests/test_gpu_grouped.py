@@ -107,6 +107,8 @@ def test_nothing_to_do():
     x, w = torch.zeros(0, 64, dtype=torch.float16, device=DEV), torch.zeros(2, 32, 64, dtype=torch.float16, device=DEV)
     assert grouped_linear(x, w, offsets([0, 0])).shape == (0, 32)
     assert grouped_linear(torch.zeros(4, 64, dtype=torch.float16, device=DEV), w[:0], offsets([])).shape == (4, 32)
+    nowhere = torch.tensor([0, -1, 5], dtype=torch.int32, device=DEV)             # no rows to pick from: rows of zeros
+    assert not bool(grouped_linear(x, w + 1, offsets([1, 2]), nowhere).any())
     idx, tw = torch.zeros(0, 2, dtype=torch.int32, device=DEV), torch.zeros(0, 2, device=DEV)
     assert dense_experts(x, idx, tw, torch.zeros(1, 64, 64, dtype=torch.float16, device=DEV), torch.zeros(1, 64, 32, dtype=torch.float16, device=DEV)).shape == (0, 64)
 
@@ -190,6 +192,20 @@ def test_dense_experts_behind_a_map(dtype):
     none = torch.full_like(g2l, -1)
     assert torch.equal(dense_experts(x, idx, w, gu, dn, global_to_local=none, residual=res), res)
     assert not bool(dense_experts(x, idx, w, gu, dn, global_to_local=none).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_held_experts_of_many(dtype):
+    """A long batch of which three of 300 experts are held here: lists much longer than what is in them."""
+    T, k, E, routed = 3000, 10, 3, 300
+    x, idx, w, gu, dn = expert_case(12, T, k, E, 64, 40, dtype, routed=routed)
+    g2l = torch.full((routed,), -1, dtype=torch.int32, device=DEV)
+    g2l[7], g2l[100], g2l[299] = 2, 0, 1
+    res = torch.randn_like(x)
+    got = dense_experts(x, idx, w, gu, dn, global_to_local=g2l, residual=res)
+    db.check(got, *experts_exact(x, idx, w, gu, dn, g2l, res), what="three of 300")
+    none = (g2l.long()[idx.long()] < 0).all(dim=1)
+    assert torch.equal(got[none], res[none])
 
 
 def test_chain_from_logits_as_a_block_runs_it():
