@@ -2,7 +2,7 @@
 //   y[t][n] = sum_k x[t][k] * scale[n][k / group] * (code[n][k] - 8)   (+ residual[t][n])
 // The code of column 8 j + i is in bits 4 i .. 4 i + 3 of word j of the row; rows are padded to whole 16 bytes.
 //
-// linear4_kernel streams the weights once per 32 tokens.  A warp takes 16 rows; lane (g, t) of it holds, for rows g and g + 8, the words of
+// linear4_kernel streams the weights once per 16 tokens.  A warp takes 16 rows; lane (g, t) of it holds, for rows g and g + 8, the words of
 // group / 4 neighbouring columns, so that one mma.sync m16n8k16 never crosses a group: contraction position is whatever order both
 // operands agree on, and x is put into that order once per CTA (shared memory, 16 bytes per lane and word).  Codes become exact
 // 16-bit numbers -8 .. 7 of x's type by mask and subtraction of a constant; products of a group are summed in fp32 by the tensor
@@ -278,10 +278,6 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   if (a.beside) grid_wait();
 }
 
-// Tokens up to which the weights are streamed; above, the tensor core's kernel.  us, bf16, groups of 128: K 2048, N 4096: 16 tokens 8.7 / 13.6, 32 tokens
-// 24 / 14; N 100003: 16 tokens 44 / 96, 32 tokens 159 / 97.
-constexpr int L4_TOKENS = 16;
-
 static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
   const int chunks = (K + L4_CHUNK - 1) / L4_CHUNK, cols = nt < 8 ? 8 : nt;
   return static_cast<size_t>((chunks + splits - 1) / splits) * (L4_CHUNK / 8) * nt * 16 + (shared_rows ? static_cast<size_t>(splits) * L4_WARPS * 16 * cols * 4 : 0);
@@ -326,36 +322,37 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
   }
   const int sms = sm_counts[dev];
   const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK, units = (a.N + (a.glu ? 7 : 15)) / (a.glu ? 8 : 16);
-  int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : a.T <= 16 ? 16 : 32;
+  int nt = a.T <= 2 ? 2 : a.T <= 8 ? 8 : 16;
   a.kwarps = 1; a.splits = 1;
   while (nt > 8 && l4_smem_bytes(nt, a.K, 8, true) > L4_SMEM_MOST) nt /= 2;
   while (a.splits < 8 && l4_smem_bytes(nt, a.K, a.splits, true) > L4_SMEM) a.splits *= 2;
-  const bool fits = l4_smem_bytes(nt, a.K, a.splits, true) <= L4_SMEM_MOST && (a.T + nt - 1) / nt <= 65535;
-  if (a.T > L4_TOKENS || !fits) {
+  // Warps of a CTA that share a row's columns: what leaves the fewest chunks one after the other.  A barrier and the pass over the parts cost a chunk and
+  // a half per row block, a cluster's barriers three: 100003 rows of 2048 columns with one, two, four and eight warps 36, 38, 44 and 59 us.
+  const int most = sms * l4_ctas(nt) / a.splits, per_split = (chunks + a.splits - 1) / a.splits;
+  double best = 1e30, round = 0.0;
+  for (int kw = 1; kw <= 8 && (kw == 1 || kw * a.splits <= chunks); kw *= 2) {
+    const int blocks = (units + L4_WARPS / kw - 1) / (L4_WARPS / kw), rounds = (blocks + most - 1) / most;
+    const double one = (per_split + kw - 1) / kw + (kw > 1 ? 1.5 : 0.3) + (a.splits > 1 ? 3.0 : 0.0);
+    if (rounds * one < best) { best = rounds * one; round = one; a.kwarps = kw; }
+  }
+  const int rws = L4_WARPS / a.kwarps;
+  a.row_blocks = (units + rws - 1) / rws;
+  const int64_t passes = (a.T + nt - 1) / nt;
+  const bool fits = l4_smem_bytes(nt, a.K, a.splits, true) <= L4_SMEM_MOST && passes <= 65535;
+  // More tokens than 16: passes over the weights side by side, or the tensor core's kernel, whichever has the smaller estimate (a wave of CTAs takes its
+  // chunks and some four us).  us in passes / on the tensor core, bf16, groups of 128: K 512, N 2048, 64 tokens 6 / 11; 2048 x 2048, 32 tokens 9 / 13 and
+  // 48 tokens 14 / 14; K 2048, N 4096, 20 tokens 13 / 14 and 32 tokens 16 / 14; 4096 x 4096, 20 tokens 19 / 17; K 2048, N 16384, 20 tokens 25 / 19.
+  const double stream_us = ((a.row_blocks * a.splits * passes + sms * l4_ctas(nt) - 1) / (sms * l4_ctas(nt))) * (round + 4.0);
+  if (!fits || (a.T > 16 && linear4_tc_us(a, sms) < stream_us)) {
     const int rc = launch_linear4_tc(a, x_dtype, group, after, st);
     if (rc != BM_ERR_UNSUPPORTED) return rc;
   }
   BM_REQUIRE(fits, BM_ERR_UNSUPPORTED, "linear4: %d rows of %d columns that do not start on 16-byte boundaries", a.T, a.K);
-  // Warps of a CTA that share a row's columns: what leaves the fewest chunks one after the other.  A barrier and the pass over the parts cost a chunk and
-  // a half per row block, a cluster's barriers three: 100003 rows of 2048 columns with one, two, four and eight warps 36, 38, 44 and 59 us.
-  const int most = sms * l4_ctas(nt) / a.splits, per_split = (chunks + a.splits - 1) / a.splits;
-  double best = 1e30;
-  for (int kw = 1; kw <= 8 && (kw == 1 || kw * a.splits <= chunks); kw *= 2) {
-    const int blocks = (units + L4_WARPS / kw - 1) / (L4_WARPS / kw), rounds = (blocks + most - 1) / most;
-    const double cost = rounds * ((per_split + kw - 1) / kw + (kw > 1 ? 1.5 : 0.3) + (a.splits > 1 ? 3.0 : 0.0));
-    if (cost < best) { best = cost; a.kwarps = kw; }
-  }
-  const int rws = L4_WARPS / a.kwarps;
-  a.row_blocks = (units + rws - 1) / rws;
   const int grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
-  const dim3 g(grid, (a.T + nt - 1) / nt);
+  const dim3 g(grid, static_cast<unsigned>(passes));
   const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
-  switch (nt) {
-    case 2: return l4_launch<2>(a, x_dtype, group, g, smem, after, st);
-    case 8: return l4_launch<8>(a, x_dtype, group, g, smem, after, st);
-    case 16: return l4_launch<16>(a, x_dtype, group, g, smem, after, st);
-    default: return l4_launch<32>(a, x_dtype, group, g, smem, after, st);
-  }
+  return nt == 2 ? l4_launch<2>(a, x_dtype, group, g, smem, after, st) : nt == 8 ? l4_launch<8>(a, x_dtype, group, g, smem, after, st)
+                                                                               : l4_launch<16>(a, x_dtype, group, g, smem, after, st);
 }
 
 }  // namespace bm

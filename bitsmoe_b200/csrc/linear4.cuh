@@ -74,6 +74,7 @@ __device__ __forceinline__ void linear4_finish(const Linear4Args& a, int row, co
 }
 
 // BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies.
+double linear4_tc_us(const Linear4Args& a, int sms);       // its time, roughly
 int launch_linear4_tc(const Linear4Args& a, int x_dtype, int group, LaunchAfter after, cudaStream_t st);
 
 }  // namespace bm

@@ -325,6 +325,16 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   if (warp == 2) tc::tmem_dealloc(tmem_base, 512);
 }
 
+// CTAs that share a tile's columns where there are few tiles (a cluster of four leaves a few SMs of a group unused).
+static int lt_splits(int64_t tiles, int slices, int sms) { return tiles * 4 <= sms * 7 / 8 && slices >= 8 ? 4 : tiles * 2 <= sms && slices >= 4 ? 2 : 1; }
+
+double linear4_tc_us(const Linear4Args& a, int sms) {
+  const int rows = a.glu ? LT_ROWS / 2 : LT_ROWS, slices = (a.K + LT_K - 1) / LT_K;
+  const int64_t tiles = static_cast<int64_t>((a.N + rows - 1) / rows) * ((a.T + LT_TOK - 1) / LT_TOK);
+  const int splits = lt_splits(tiles, slices, sms);
+  return 9.0 + 0.45 * ((slices + splits - 1) / splits) * ((tiles * splits + sms - 1) / sms);
+}
+
 int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAfter after, cudaStream_t st) {
   const Linear4Args& a = args;
   if (a.ldx % 8 != 0 || !aligned16(a.x, a.p[0], a.p[1])) return BM_ERR_UNSUPPORTED;
@@ -359,11 +369,8 @@ int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAft
     BM_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     once.mark(dev);
   }
-  // few tiles: clusters of two or four CTAs share the columns of one (a cluster of four leaves a few SMs of a group unused)
   const int tiles = p.row_tiles * p.tok_tiles;
-  p.splits = 1;
-  if (tiles * 4 <= sms[dev] * 7 / 8 && p.slices >= 8) p.splits = 4;
-  else if (tiles * 2 <= sms[dev] && p.slices >= 4) p.splits = 2;
+  p.splits = lt_splits(tiles, p.slices, sms[dev]);
   const int grid = p.splits > 1 ? tiles * p.splits : tiles < sms[dev] ? tiles : sms[dev];
   auto* kernel = x_dtype == BM_F16 ? (a.glu ? linear4_tc_kernel<BM_F16, true> : linear4_tc_kernel<BM_F16, false>)
                                    : (a.glu ? linear4_tc_kernel<BM_BF16, true> : linear4_tc_kernel<BM_BF16, false>);

@@ -111,6 +111,19 @@ def test_shapes(tokens, n, k, group, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", q4.GROUP_SIZES)
+@pytest.mark.parametrize("n,k", [(4100, 4096), (2057, 8192), (20001, 1100)])
+@pytest.mark.parametrize("tokens", [17, 24, 33, 64, 131])
+def test_matrices_too_large_for_passes(tokens, n, k, group, dtype):
+    """Sizes at which more than 16 tokens go to the tensor core: columns shared by two and four CTAs and whole, ends in every direction."""
+    gen = torch.Generator().manual_seed(n + tokens)
+    m, w = matrix4(gen, n, k, group)
+    x, res = rnd(gen, tokens, k, dtype=dtype), rnd(gen, tokens, n, dtype=dtype)
+    db.check(linear4(x, *m, group, residual=res), *exact(x, w, res), what="linear4")
+
+
+@gpu
 @pytest.mark.parametrize("tokens", [3, 100])
 def test_values_far_from_one(tokens):
     """bf16 activations beyond fp16's range, infinities in one row, rows of zeros, scales of zero and subnormal scales."""
@@ -182,6 +195,13 @@ def test_strided_and_unaligned_rows():
     res = rnd(gen, 40, 6).t()
     db.check(linear4(flat, *m, 32, residual=res), *exact(flat, w, res.half()), what="strided fp32 residual")
     assert linear4(flat[:0], *m, 32).shape == (0, 40)
+
+
+@gpu
+@pytest.mark.parametrize("tokens,hidden,inter", [(33, 2056, 4100), (150, 4096, 2050)])
+def test_mlp_on_the_tensor_core(tokens, hidden, inter):
+    x, packs, mats, tg, res = mlp_case(inter, tokens, hidden, inter, 128, torch.bfloat16)
+    db.check(dense_mlp4(x, *packs, 128, token_gate_weight=tg, residual=res), *mlp_exact(x, mats, tg, res), what="mlp4")
 
 
 @gpu
