@@ -13,6 +13,7 @@ tables built once per block), routing is built by one kernel without a device->h
 """
 from __future__ import annotations
 
+import threading
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -23,6 +24,7 @@ from bitsmoe_b200.quant.linear4 import Linear4
 
 _FIELDS = ("payload", "rank_idx", "tile_meta", "slab_meta", "scale", "s")
 _TAGS = ("gate", "up", "down")
+_STACKING = threading.Lock()      # one for all blocks: an expert may belong to several, and a block is copied and pickled without it
 
 
 class BitsMoE_BaseSparseMoeBlock(nn.Module):
@@ -212,29 +214,51 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
 
     def _stacked_super_weights(self) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         """The un-quantised experts' weights as two stacked tensors, whose slices the experts' own parameters become: nothing is held
-        twice, and what is written to a parameter is what the kernels read.  Built again once a parameter lives somewhere else."""
+        twice, and what is written to a parameter is what the kernels read.  Built again once a parameter lives somewhere else; whoever
+        builds it waits for the device, as the packed part of the cache does."""
         parts = self._super_parts()
         if parts is None:
             return None
-        inter, hidden = parts[0][0].shape
-        held = self._super_weights
-        if held is not None:
-            gu, dn = held
-            where = [(gu[i, :inter], gu[i, inter:], dn[i]) for i in range(len(parts))]
-            if gu.shape == (len(parts), 2 * inter, hidden) and all(p.data_ptr() == v.data_ptr() and p.is_contiguous() for w, vs in zip(parts, where) for p, v in zip(w, vs)):
-                return held
-        first = parts[0][0]
-        if first.is_cuda and torch.cuda.is_current_stream_capturing():
-            return None                          # the copies would run at the graph's replay
-        with torch.inference_mode(False), torch.no_grad():        # the parameters stay ordinary tensors, whatever mode the first call is in
-            gu = torch.empty((len(parts), 2 * inter, hidden), dtype=first.dtype, device=first.device)
-            dn = torch.empty((len(parts), hidden, inter), dtype=first.dtype, device=first.device)
-            for i, w in enumerate(parts):
-                for p, v in zip(w, (gu[i, :inter], gu[i, inter:], dn[i])):
-                    v.copy_(p)
-                    p.data = v
-        self._super_weights = (gu, dn)
+        if self._stack_holds(parts):
+            return self._super_weights
+        device = parts[0][0].device
+        if device.type == "cuda":
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    return None                  # the copies would run at the graph's replay
+        with _STACKING:
+            if not self._stack_holds(parts):     # else another thread has just built it
+                inter, hidden = parts[0][0].shape
+                with torch.inference_mode(False), torch.no_grad():    # the parameters stay ordinary tensors, whatever mode the first call is in
+                    gu = parts[0][0].new_empty((len(parts), 2 * inter, hidden))
+                    dn = parts[0][0].new_empty((len(parts), hidden, inter))
+                    views = [(gu[i, :inter], gu[i, inter:], dn[i]) for i in range(len(parts))]
+                    for w, vs in zip(parts, views):
+                        for p, v in zip(w, vs):
+                            v.copy_(p)
+                    self._finish_copies(device)
+                    for w, vs in zip(parts, views):
+                        for p, v in zip(w, vs):
+                            p.data = v
+                self._super_weights = (gu, dn)
         return self._super_weights
+
+    def _stack_holds(self, parts) -> bool:
+        """Whether the experts' parameters are the slices of the stack."""
+        if self._super_weights is None:
+            return False
+        gu, dn = self._super_weights
+        inter, hidden = parts[0][0].shape
+        return (gu.shape == (len(parts), 2 * inter, hidden) and
+                all(p.data_ptr() == v.data_ptr() and p.is_contiguous()
+                    for i, w in enumerate(parts) for p, v in zip(w, (gu[i, :inter], gu[i, inter:], dn[i]))))
+
+    @staticmethod
+    def _finish_copies(device: torch.device) -> None:
+        """Calls on other streams use the slices as soon as they are the parameters, and the storage that the parameters leave goes back
+        to the stream that it was made on: both have to wait until the copies are done, and what reads the old storage with them."""
+        if device.type == "cuda":
+            torch.cuda.synchronize(device)
 
     def _library_super_experts(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
                                residual: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
