@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from bitsmoe_b200.algorithms import _HAS_MLP_FORWARD_CUDA, mlp_forward_cuda
+from bitsmoe_b200.models.swiglu import runs_as_swiglu
 from bitsmoe_b200.quant.linear4 import Linear4
 
 _FIELDS = ("payload", "rank_idx", "tile_meta", "slab_meta", "scale", "s")
@@ -200,8 +201,10 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
             return None
         parts = []
         for _, module in self._super_expert_items:
-            w = [self._bare_weight(getattr(module, n, None)) for n in ("gate_proj", "up_proj", "down_proj")]
-            if any(p is None for p in w):
+            if not runs_as_swiglu(module):
+                return None
+            w = [module._modules[n]._parameters.get("weight") for n in ("gate_proj", "up_proj", "down_proj")]
+            if any(type(p) is not nn.Parameter for p in w):
                 return None
             parts.append(w)
         g = parts[0][0]
@@ -333,7 +336,7 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         sigmoid(token_gate(x)) when a one-output bias-free Linear is given; None when the module is of another kind."""
         parts = [getattr(mlp, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
         if all(isinstance(p, Linear4) for p in parts):
-            return self._library_dense_mlp4(x, parts, token_gate)
+            return self._library_dense_mlp4(x, parts, token_gate) if runs_as_swiglu(mlp) else None
         if not (x.is_cuda and all(self._plain_linear(p) for p in parts) and not torch.is_grad_enabled()):
             return None
         if token_gate is not None and not (self._plain_linear(token_gate) and token_gate.weight.shape[0] == 1):

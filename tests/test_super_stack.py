@@ -97,3 +97,128 @@ def test_first_call_on_a_side_stream():
     assert all(torch.equal(w, k) for w, k in zip((w for e in (2, 5) for w in weights(blk.experts[e])), kept))
     helpers.assert_close(a, want, what="first stream")
     helpers.assert_close(b, want, what="second stream")
+
+
+# ---- which modules the library stands in for
+class Gelu(DenseMLP):
+    def forward(self, x):
+        return self.down_proj(nn.functional.gelu(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Clamped(DenseMLP):
+    def forward(self, x):
+        return self.down_proj(nn.functional.silu(self.gate_proj(x)).clamp(max=7.0) * self.up_proj(x))
+
+
+class Swapped(DenseMLP):
+    def forward(self, x):
+        return self.down_proj(self.gate_proj(x) * nn.functional.silu(self.up_proj(x)))
+
+
+class Scaled(DenseMLP):
+    def forward(self, x):
+        return self.down_proj(nn.functional.silu(self.gate_proj(x)) * self.up_proj(x)) * 0.5
+
+
+class Counting(DenseMLP):
+    calls = 0
+
+    def forward(self, x):
+        self.calls += 1
+        return DenseMLP.forward(self, x)
+
+
+class Noisy(DenseMLP):
+    def forward(self, x):
+        h = self.up_proj(x) * nn.functional.silu(self.gate_proj(x))
+        return self.down_proj(h + torch.randn_like(h) if self.noise else h)
+
+
+class WithAct(DenseMLP):
+    def __init__(self, hidden, inter, act):
+        super().__init__(hidden, inter)
+        self.act_fn = act
+
+    def forward(self, x):
+        return self.down_proj(torch.mul(self.act_fn(self.gate_proj(x)), self.up_proj(x)))
+
+
+class LowRankLinear(nn.Linear):
+    def forward(self, x):
+        return super().forward(x) + x.sum(dim=-1, keepdim=True)
+
+
+def low_rank():
+    m = mlp()
+    m.up_proj = LowRankLinear(HIDDEN, INTER, bias=False).half()
+    return m
+
+
+def hooked(name=None, pre=False):
+    m = mlp()
+    on = m if name is None else getattr(m, name)
+    on.register_forward_pre_hook(lambda mod, a: None) if pre else on.register_forward_hook(lambda mod, a, out: out * 2)
+    return m
+
+
+def forward_of_its_own():
+    m = mlp()
+    m.forward = lambda x: x
+    return m
+
+
+OTHER_KINDS = {
+    "another activation in its forward": lambda: Gelu(HIDDEN, INTER).half(), "a clamp": lambda: Clamped(HIDDEN, INTER).half(),
+    "gate and up the other way round": lambda: Swapped(HIDDEN, INTER).half(), "a factor": lambda: Scaled(HIDDEN, INTER).half(),
+    "writes to itself": lambda: Counting(HIDDEN, INTER).half(), "an activation module": lambda: WithAct(HIDDEN, INTER, nn.GELU()).half(),
+    "an activation function": lambda: WithAct(HIDDEN, INTER, torch.tanh).half(), "a Linear of another class": low_rank, "a hook": hooked,
+    "a hook on a Linear": lambda: hooked("down_proj"), "a hook before it": lambda: hooked(pre=True), "a forward of its own": forward_of_its_own,
+}
+
+
+@pytest.mark.parametrize("kind", OTHER_KINDS)
+def test_modules_of_another_kind_are_not_stacked(kind):
+    other = OTHER_KINDS[kind]()
+    blk = host_block({1: mlp(1), 4: other})
+    where = [w.data_ptr() for w in weights(other)]
+    assert blk._stacked_super_weights() is None and [w.data_ptr() for w in weights(other)] == where
+
+
+def test_modules_that_are_swiglu_are_stacked():
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeMLP
+    conf = NS(hidden_size=HIDDEN, intermediate_size=INTER, hidden_act="silu")
+    kinds = [mlp(), Qwen3MoeMLP(conf).half(), WithAct(HIDDEN, INTER, nn.SiLU()).half(), WithAct(HIDDEN, INTER, nn.functional.silu).half()]
+    assert host_block(dict(enumerate(kinds)))._stacked_super_weights()[0].shape == (4, 2 * INTER, HIDDEN)
+
+
+def test_changes_of_a_module_are_noticed():
+    act, noisy = WithAct(HIDDEN, INTER, nn.SiLU()).half(), Noisy(HIDDEN, INTER).half()
+    noisy.noise = False
+    blk = host_block({1: act, 4: noisy})
+    assert blk._stacked_super_weights() is not None
+    for change, back in ((lambda: setattr(act, "act_fn", nn.GELU()), lambda: setattr(act, "act_fn", nn.SiLU())),
+                         (lambda: setattr(noisy, "noise", True), lambda: setattr(noisy, "noise", False))):
+        change()
+        assert blk._stacked_super_weights() is None
+        back()
+        assert blk._stacked_super_weights() is not None
+    for on in (act, act.gate_proj, act.act_fn):
+        handle = on.register_forward_hook(lambda *a: None)
+        assert blk._stacked_super_weights() is None
+        handle.remove()
+        assert blk._stacked_super_weights() is not None
+
+
+def test_a_shared_expert_of_another_kind_keeps_its_forward_in_4_bits(monkeypatch):
+    """What holds a Linear in 4 bits does not make a SwiGLU of its MLP."""
+    from bitsmoe_b200.quant.linear4 import Linear4
+    blk = host_block({1: mlp(1)})
+    ran = []
+    monkeypatch.setattr(blk, "_library_dense_mlp4", lambda *a: ran.append(1) or a[0])
+    x = torch.zeros(3, HIDDEN, dtype=torch.float16)
+    for kind, runs in ((DenseMLP, 1), (Gelu, 0)):
+        m = kind(HIDDEN, INTER)
+        for n in ("gate_proj", "up_proj", "down_proj"):
+            setattr(m, n, Linear4.from_linear(getattr(m, n), 32))
+        del ran[:]
+        assert (blk._library_dense_mlp(x, m) is not None) == bool(runs) and len(ran) == runs
