@@ -118,7 +118,6 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         if layer is not None:
             layer.close()
         self._packed_layer = None
-        self._super_weights = None
 
     def _ensure_runtime_cache(self, device: torch.device) -> None:
         if self._runtime_cache_ready and self._runtime_cache_device == device:
@@ -146,6 +145,8 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         for local, (idx, _) in enumerate(super_items):
             supers[idx] = local
         self._super_global_to_local = supers.to(device) if super_items else None
+        if not super_items:
+            self._super_weights = None           # otherwise the parameters are its slices as long as they live where they do
         self._identity_map = self._packed_expert_count == self.num_experts and not super_items
         modules = [m for _, m in packed_items]
         for tag in _TAGS:

@@ -75,6 +75,41 @@ def test_threads_in_their_first_call_share_one_stack(monkeypatch):
     assert all(torch.equal(a, v) for a, v in zip((w for e in (1, 4, 6) for w in weights(blk.experts[e])), values))
 
 
+def test_loading_weights_keeps_the_stack():
+    """What is loaded goes into the slices: the stack that a captured graph reads stays the one in use."""
+    blk = host_block({1: mlp(1), 4: mlp(2)})
+    gu, dn = blk._stacked_super_weights()
+    doubled = {k: v * 2 if "experts" in k else v for k, v in blk.state_dict().items()}
+    blk.load_state_dict(doubled)
+    blk._ensure_runtime_cache(torch.device("cpu"))
+    again = blk._stacked_super_weights()
+    assert again[0] is gu and again[1] is dn and torch.equal(gu[1, :INTER], doubled["experts.4.gate_proj.weight"])
+    blk.set_expert(4, mlp(3), packed=False)                  # another module: another stack
+    blk._ensure_runtime_cache(torch.device("cpu"))
+    assert blk._stacked_super_weights()[0] is not gu
+
+
+@gpu
+def test_a_captured_block_follows_loaded_weights():
+    cfg, blk = _qwen_block([1, 2])
+    x = torch.randn(1, 24, cfg.hidden, generator=torch.Generator().manual_seed(2)).to(DEV).half()
+    with torch.no_grad():
+        blk(x)
+        stack = blk._super_weights
+        idx = torch.tensor([[1, 2]], dtype=torch.int32, device=DEV).expand(24, 2).contiguous()
+        w = torch.full((24, 2), 0.5, device=DEV)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = blk._library_super_experts(x[0], idx, w, None)
+        state = {k: v * 0.5 if "experts.2.up_proj" in k else v for k, v in blk.state_dict().items()}
+        blk.load_state_dict(state)
+        blk(x)
+        assert blk._super_weights is stack
+        g.replay()
+        torch.cuda.synchronize()
+        helpers.assert_close(out, sum(0.5 * blk.experts[e](x[0]).float() for e in (1, 2)), what="replayed experts")
+
+
 @gpu
 def test_first_call_on_a_side_stream():
     """Weights are loaded on one stream, the first call runs on another that is behind with its work, a third uses the block right
