@@ -225,6 +225,8 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
             return None
         if self._stack_holds(parts):
             return self._super_weights
+        if not self._can_stack(parts):
+            return None
         device = parts[0][0].device
         if device.type == "cuda":
             with torch.cuda.device(device):
@@ -256,6 +258,15 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         return (gu.shape == (len(parts), 2 * inter, hidden) and
                 all(p.data_ptr() == v.data_ptr() and p.is_contiguous()
                     for i, w in enumerate(parts) for p, v in zip(w, (gu[i, :inter], gu[i, inter:], dn[i]))))
+
+    def _can_stack(self, parts) -> bool:
+        """Whether every parameter has a storage of its own, or is a slice of this block's stack: moving one that others look into (an
+        expert that several ids or blocks share, a view of a larger tensor) would part them, and move it back and forth."""
+        held = () if self._super_weights is None else tuple(t.untyped_storage().data_ptr() for t in self._super_weights)
+        flat = [p for w in parts for p in w]
+        if len({p.data_ptr() for p in flat}) != len(flat):
+            return False
+        return all(p.untyped_storage().data_ptr() in held or p.untyped_storage().nbytes() == p.numel() * p.element_size() for p in flat)
 
     @staticmethod
     def _finish_copies(device: torch.device) -> None:

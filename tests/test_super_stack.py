@@ -89,6 +89,34 @@ def test_loading_weights_keeps_the_stack():
     assert blk._stacked_super_weights()[0] is not gu
 
 
+def test_shared_parameters_stay_where_they_are():
+    """Ids, or blocks, that share an expert: each would move the parameters to a stack of its own in every call."""
+    m = mlp(1)
+    blk = host_block({1: m, 4: m})
+    before = [w.data_ptr() for w in weights(m)]
+    for _ in range(2):
+        assert blk._stacked_super_weights() is None and [w.data_ptr() for w in weights(m)] == before
+    first, second = host_block({1: m}), host_block({2: m, 3: mlp(2)})
+    gu, _ = first._stacked_super_weights()
+    for _ in range(2):
+        assert second._stacked_super_weights() is None and first._stacked_super_weights()[0] is gu
+    fused = torch.randn(2 * INTER, HIDDEN).half()
+    views = mlp(3)
+    views.gate_proj.weight, views.up_proj.weight = (nn.Parameter(v) for v in fused.chunk(2))
+    assert host_block({0: views})._stacked_super_weights() is None and views.up_proj.weight.data_ptr() == fused[INTER].data_ptr()
+
+
+def test_one_parameter_that_moved_is_taken_back():
+    a, b = mlp(1), mlp(2)
+    blk = host_block({1: a, 4: b})
+    blk._stacked_super_weights()
+    want = [w.detach().clone() for m in (a, b) for w in weights(m)]
+    want[5] *= 2
+    b.down_proj.weight.data = b.down_proj.weight.data * 2
+    gu, dn = blk._stacked_super_weights()
+    assert all(torch.equal(w, v) for w, v in zip((w for m in (a, b) for w in weights(m)), want)) and torch.equal(dn[1], want[5])
+
+
 @gpu
 def test_a_captured_block_follows_loaded_weights():
     cfg, blk = _qwen_block([1, 2])
