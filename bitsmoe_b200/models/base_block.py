@@ -211,8 +211,12 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         g = parts[0][0]
         if g.dtype not in (torch.float16, torch.bfloat16):
             return None
-        for w in parts:
-            if w[0].shape != g.shape or w[1].shape != g.shape or w[2].shape != g.shape[::-1] or any(p.dtype != g.dtype or p.device != g.device for p in w):
+        shape, dtype, device = g.shape, g.dtype, g.device
+        back = shape[::-1]
+        for gate, up, down in parts:
+            if gate.shape != shape or up.shape != shape or down.shape != back:
+                return None
+            if gate.dtype != dtype or up.dtype != dtype or down.dtype != dtype or gate.device != device or up.device != device or down.device != device:
                 return None
         return parts
 
@@ -255,9 +259,17 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
             return False
         gu, dn = self._super_weights
         inter, hidden = parts[0][0].shape
-        return (gu.shape == (len(parts), 2 * inter, hidden) and
-                all(p.data_ptr() == v.data_ptr() and p.is_contiguous()
-                    for i, w in enumerate(parts) for p, v in zip(w, (gu[i, :inter], gu[i, inter:], dn[i]))))
+        if gu.shape != (len(parts), 2 * inter, hidden):
+            return False
+        # addresses, not views: this runs in every call
+        size, at, down = inter * hidden * gu.element_size(), gu.data_ptr(), dn.data_ptr()
+        for gate, up, dwn in parts:
+            if gate.data_ptr() != at or up.data_ptr() != at + size or dwn.data_ptr() != down:
+                return False
+            if not (gate.is_contiguous() and up.is_contiguous() and dwn.is_contiguous()):
+                return False
+            at, down = at + 2 * size, down + size
+        return True
 
     def _can_stack(self, parts) -> bool:
         """Whether every parameter has a storage of its own, or is a slice of this block's stack: moving one that others look into (an

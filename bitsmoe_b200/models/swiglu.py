@@ -8,6 +8,7 @@ module) makes it another kind of module, which the block then calls as it is.
 """
 from __future__ import annotations
 
+import operator
 import weakref
 
 import torch
@@ -93,9 +94,15 @@ def runs_as_swiglu(module) -> bool:
                 return False
         elif type(m) is not Linear4:
             return False
-    state = (type(module).forward, *(v for k, v in module.__dict__.items() if k[0] != "_"), *children.values())
+    attributes = module.__dict__
+    state = [type(module).forward, *children.values(), *[attributes[k] for k in attributes if k[0] != "_"]]
     known = _TRACED.get(module)
-    if known is None or len(known[0]) != len(state) or any(a is not b for a, b in zip(known[0], state)):
+    if known is None or len(known[0]) != len(state) or not all(map(operator.is_, known[0], state)):
         known = (state, _traces_as_swiglu(module))
         _TRACED[module] = known
-    return known[1] and not any(_hooked(m) for m in children.values() if m is not None)
+    if not known[1]:
+        return False
+    for m in children.values():
+        if m is not None and (m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__):
+            return False
+    return True
