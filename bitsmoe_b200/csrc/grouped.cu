@@ -94,8 +94,12 @@ __global__ void __launch_bounds__(GG_THREADS) grouped_any_kernel(const GroupedAr
     if (n0 + col < a.N)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (4 * rg + j < rows)
-          store_act(a.y, a.y_dtype, static_cast<int64_t>(row0 + 4 * rg + j) * a.N + n0 + col, GLU ? silu_mul(acc[0][j], acc[GLU ? 1 : 0][j]) : acc[0][j]);
+        if (4 * rg + j < rows) {
+          const int64_t o = static_cast<int64_t>(row0 + 4 * rg + j) * a.N + n0 + col;
+          const float v = GLU ? silu_mul(acc[0][j], acc[GLU ? 1 : 0][j]) : acc[0][j];
+          store_act(a.y, a.y_dtype, o, v);
+          if (GLU && D == BM_F16 && a.wide && !fits_fp16(v)) a.wide[o] = v;
+        }
     __syncthreads();
   }
 }
@@ -172,7 +176,25 @@ struct CombineArgs {
   const void* residual;
   void* y;
   int k, H, vec;               // vec: H % 4 == 0, y and the residual on 8-byte boundaries
+  // fp16: what the down product was made of
+  SlotArgs slots;
+  const void *z, *w_down;      // [rows, I], [E, H, I]
+  const float* wide;           // [rows, I], valid where z is not finite
+  int I;
 };
+// A column of a row of d from z's values before their rounding.  The product between the two matrices of an expert may pass fp16's range
+// where the sum over it does not: z is infinite there, and with it the row of d.
+__device__ __forceinline__ float wide_down(const CombineArgs& a, int slot, int64_t at, int h) {
+  const __half *z = static_cast<const __half*>(a.z) + at * a.I, *w = static_cast<const __half*>(a.w_down) + (static_cast<int64_t>(slot_expert(a.slots, slot)) * a.H + h) * a.I;
+  float v = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < a.I; ++i) {
+    float f = __half2float(z[i]);
+    if (!(fabsf(f) <= 65504.f)) f = a.wide[at * a.I + i];
+    v = fmaf(__half2float(w[i]), f, v);
+  }
+  return v;
+}
 template <int D>
 __device__ __forceinline__ float4 load4(const void* p, int64_t i) {
   const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
@@ -223,6 +245,21 @@ __global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const Combi
       v[3] = fmaf(w[u], d[u].w, v[3]);
     }
   }
+  if (D == BM_F16 && !(fabsf((v[0] + v[1]) + (v[2] + v[3])) < __int_as_float(0x7f800000)))
+    // once more, slot by slot, with the rows of d that are not finite worked out anew
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      float sum = a.residual ? load16<D>(a.residual, o + j) : 0.f;
+#pragma unroll 1
+      for (int s = 0; s < a.k; ++s) {
+        const int slot = t * a.k + s, at = a.pos[slot];
+        if (at < 0) continue;
+        float d = a.d[static_cast<int64_t>(at) * a.H + h + j];
+        if (!(fabsf(d) < __int_as_float(0x7f800000))) d = wide_down(a, slot, at, h + j);
+        sum = fmaf(a.topk_w[slot], d, sum);
+      }
+      v[0] = j == 0 ? sum : v[0]; v[1] = j == 1 ? sum : v[1]; v[2] = j == 2 ? sum : v[2]; v[3] = j == 3 ? sum : v[3];
+    }
   uint16_t out[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = D == BM_F16 ? __half_as_ushort(__float2half_rn(v[j])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
@@ -232,7 +269,7 @@ __global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const Combi
 }
 
 struct DenseExpertsWs {
-  size_t tok, rw, pos, off, route, xs, z, d, total;
+  size_t tok, rw, pos, off, route, xs, z, wide, d, total;
   DenseExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
     const size_t A = static_cast<size_t>(T * k);
     size_t at = 0;
@@ -247,6 +284,7 @@ struct DenseExpertsWs {
     off = take(static_cast<size_t>(E + 1) * 4);
     route = take(bm_route_build_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(k), static_cast<int32_t>(E)));
     z = take(A * I * 2);
+    wide = take(A * I * 4);
     d = xs = take(A * H * 4);      // rows of x in expert order are read before the down products are written
     total = at;
   }
@@ -312,6 +350,7 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
   g.x_rows = T; g.rows = A; g.K = hidden; g.N = intermediate; g.E = num_local; g.dtype = g.y_dtype = dtype; g.glu = 1;
   g.expected = static_cast<int>(static_cast<int64_t>(A) * num_local / std::max(num_routed, num_local));
   g.gathered = ws + at.xs;
+  g.wide = dtype == BM_F16 ? reinterpret_cast<float*>(ws + at.wide) : nullptr;
   g.after = AFTER_READS;
   if ((rc = launch_grouped(g, st))) return rc;
   g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
@@ -322,6 +361,7 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
   CombineArgs c{};
   c.d = reinterpret_cast<const float*>(ws + at.d);
   c.pos = pos; c.topk_w = topk_w; c.residual = residual; c.y = y; c.k = k; c.H = hidden;
+  c.slots = g.slots; c.z = ws + at.z; c.wide = reinterpret_cast<const float*>(ws + at.wide); c.w_down = w_down; c.I = intermediate;
   c.vec = hidden % 4 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 7u) == 0;
   BM_CUDA(launch_after(AFTER_READS, 1, dtype == BM_F16 ? experts_combine_kernel<BM_F16> : experts_combine_kernel<BM_BF16>,
                        dim3(T, (hidden + 4 * EC_THREADS - 1) / (4 * EC_THREADS)), EC_THREADS, 0, st, c));

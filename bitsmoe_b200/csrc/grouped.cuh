@@ -25,6 +25,7 @@ struct GroupedArgs {
   int x_rows, rows, K, N, E;
   int dtype, y_dtype;          // of x and w: BM_F16 or BM_BF16; of y: the same or BM_F32
   int glu;
+  float* wide;                 // glu with fp16 y: [rows, N], gets the values that fp16 does not hold (their y is infinite); or null
   int expected;                // rows that the groups are expected to have, 0 = `rows`
   void* gathered;              // with an index: room for [rows, K], 16-byte aligned, or null
   SlotArgs slots;              // worked out beside the products
@@ -60,6 +61,9 @@ __device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int ro
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+// Whether rounding v to fp16 leaves a number (65520 is half way from the largest one to the next power of two).
+__device__ __forceinline__ bool fits_fp16(float v) { return fabsf(v) < 65520.f; }
 
 // BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies (grouped_tc.cu).
 int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st);

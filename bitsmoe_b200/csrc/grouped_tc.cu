@@ -43,6 +43,7 @@ struct GcParams {
   const int32_t* offsets;
   const int32_t* index;
   void* y;
+  float* wide;
   int x_rows, rows, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
   SlotArgs slots;
 };
@@ -372,6 +373,17 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         if (GLU) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) lo[i] = __float_as_uint(silu_mul(__uint_as_float(lo[i]), __uint_as_float(hi[i])));
+          if (!BF16 && p.wide) {
+            bool fits = true;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fits &= fits_fp16(__uint_as_float(lo[i]));
+            if (!fits)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int r = c0 + 8 * (i >> 2) + 2 * (lane & 3) + (i & 1), col = col0 + (lane >> 2) + 8 * ((i >> 1) & 1);
+                if (!fits_fp16(__uint_as_float(lo[i])) && r < it.rows && col < p.N) p.wide[static_cast<int64_t>(it.row0 + r) * p.N + col] = __uint_as_float(lo[i]);
+              }
+          }
         }
 #pragma unroll
         for (int h = 0; h < (GLU ? 1 : 2); ++h) {
@@ -444,7 +456,7 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
     const cuuint32_t box[3] = {GC_K, 128, 1}, box32[3] = {GC_K, 32, 1};
     if (!encode_map16(&p.w, a.w, 3, dims, strides, box) || !encode_map16(&p.w32, a.w, 3, dims, strides, box32)) return BM_ERR_UNSUPPORTED;
   }
-  p.offsets = a.offsets; p.index = a.index; p.y = a.y;
+  p.offsets = a.offsets; p.index = a.index; p.y = a.y; p.wide = a.wide;
   p.x_rows = a.x_rows; p.rows = a.rows; p.N = a.N; p.E = a.E;
   p.slices = (a.K + GC_K - 1) / GC_K;
   p.vec = a.N % 8 == 0 && aligned16(a.y);

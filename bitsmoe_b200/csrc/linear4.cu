@@ -58,10 +58,14 @@ __device__ __forceinline__ uint4 l4_stream(const uint4* p) {
   return v;
 }
 
-template <int NT, int XD, int WPL>
+// WIDE: one of the two products of an fp16 MLP, whose middle may pass fp16's range; its few instructions on the way out cost products that have
+// no need of them 2 to 7 %.
+template <int NT, int XD, int WPL, bool WIDE>
 __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const __grid_constant__ Linear4Args a) {
   constexpr int NB = NT < 8 ? 1 : NT / 8, GPC = 4 / WPL, L4_BATCH = l4_batch(NT), SPR = (L4_BATCH * GPC + 3) / 4;     // groups a chunk, scale loads per row and batch
   extern __shared__ __align__(16) unsigned char l4_smem[];
+  __shared__ int left_out;                 // linear4_finish
+  if (WIDE && threadIdx.x == 0) left_out = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % a.splits, kw = warp % a.kwarps, rw = warp / a.kwarps, rws = L4_WARPS / a.kwarps;
   const int chunks = (a.K + L4_CHUNK - 1) / L4_CHUNK;
@@ -217,11 +221,11 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
         auto token = [&](int row, int i) { return 8 * b + 2 * t + i < nn && row < a.N ? n0 + 8 * b + 2 * t + i : -1; };
         if (a.glu) {
           const float z[2] = {silu_mul(acc[b][0], acc[b][2]), silu_mul(acc[b][1], acc[b][3])};
-          linear4_finish<XD>(a, ra, z, [&](int i) { return token(ra, i); });
+          linear4_finish<XD, WIDE>(a, ra, z, left_out, [&](int i) { return token(ra, i); });
         } else {
           const float lo[2] = {acc[b][0], acc[b][1]}, hi[2] = {acc[b][2], acc[b][3]};
-          linear4_finish<XD>(a, ra, lo, [&](int i) { return token(ra, i); });
-          linear4_finish<XD>(a, rc, hi, [&](int i) { return token(rc, i); });
+          linear4_finish<XD, WIDE>(a, ra, lo, left_out, [&](int i) { return token(ra, i); });
+          linear4_finish<XD, WIDE>(a, rc, hi, left_out, [&](int i) { return token(rc, i); });
         }
       }
       return;
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
             if (a.glu) u += part[(row + 8) * COLS];
           }
         const float out[1] = {a.glu ? silu_mul(v, u) : v};
-        linear4_finish<XD>(a, out_row, out, [&](int) { return n0 + n; });
+        linear4_finish<XD, WIDE>(a, out_row, out, left_out, [&](int) { return n0 + n; });
       }
     }
     if (a.splits == 1) __syncthreads();                  // the parts may be overwritten
@@ -275,6 +279,11 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   };
   while (step(w[0], sv[0], w[1], sv[1]) && step(w[1], sv[1], w[0], sv[0])) {
   }
+  if (WIDE && a.x_wide) {
+    __syncthreads();
+    if (left_out)
+      for (rb = cluster_id; rb < a.row_blocks; rb += clusters) linear4_redo(a, rb * rws * 16, rws * 16, n0, nn);
+  }
   if (a.beside) grid_wait();
 }
 
@@ -283,33 +292,35 @@ static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
   return static_cast<size_t>((chunks + splits - 1) / splits) * (L4_CHUNK / 8) * nt * 16 + (shared_rows ? static_cast<size_t>(splits) * L4_WARPS * 16 * cols * 4 : 0);
 }
 
-template <int NT, int XD, int WPL>
+template <int NT, int XD, int WPL, bool WIDE>
 static int l4_launch_one(const Linear4Args& a, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
   static PerDeviceOnce once;
   int dev = -1;
   BM_CUDA(cudaGetDevice(&dev));
   if (!once.is_done(dev)) {
-    BM_CUDA(cudaFuncSetAttribute(linear4_kernel<NT, XD, WPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L4_SMEM_MOST)));
+    BM_CUDA(cudaFuncSetAttribute(linear4_kernel<NT, XD, WPL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L4_SMEM_MOST)));
     once.mark(dev);
   }
-  BM_CUDA(launch_after(after, a.splits, linear4_kernel<NT, XD, WPL>, grid, L4_THREADS, smem, st, a));
+  BM_CUDA(launch_after(after, a.splits, linear4_kernel<NT, XD, WPL, WIDE>, grid, L4_THREADS, smem, st, a));
   BM_LAUNCH_CHECK("linear4_kernel");
   return BM_OK;
 }
-template <int NT, int XD>
+template <int NT, int XD, bool WIDE>
 static int l4_launch_group(const Linear4Args& a, int group, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
-  return group == 128 ? l4_launch_one<NT, XD, 4>(a, grid, smem, after, st) : group == 64 ? l4_launch_one<NT, XD, 2>(a, grid, smem, after, st)
-                                                                                       : l4_launch_one<NT, XD, 1>(a, grid, smem, after, st);
+  return group == 128 ? l4_launch_one<NT, XD, 4, WIDE>(a, grid, smem, after, st) : group == 64 ? l4_launch_one<NT, XD, 2, WIDE>(a, grid, smem, after, st)
+                                                                                       : l4_launch_one<NT, XD, 1, WIDE>(a, grid, smem, after, st);
 }
 template <int NT>
 static int l4_launch(const Linear4Args& a, int x_dtype, int group, dim3 grid, size_t smem, LaunchAfter after, cudaStream_t st) {
-  return x_dtype == BM_F16 ? l4_launch_group<NT, BM_F16>(a, group, grid, smem, after, st) : l4_launch_group<NT, BM_BF16>(a, group, grid, smem, after, st);
+  if (x_dtype == BM_BF16) return l4_launch_group<NT, BM_BF16, false>(a, group, grid, smem, after, st);
+  return a.wide || a.x_wide ? l4_launch_group<NT, BM_F16, true>(a, group, grid, smem, after, st) : l4_launch_group<NT, BM_F16, false>(a, group, grid, smem, after, st);
 }
 
 // y = x . W^T, or with glu z = silu(x . Wg^T) * (x . Wu^T).
 static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cudaStream_t st) {
   a.words = (a.K + 31) / 32 * 4;
   a.groups = (a.K + group - 1) / group;
+  a.group = group;
   a.vec_x = aligned16(a.x) && a.ldx % 8 == 0;
   static PerDeviceOnce once;
   static int sm_counts[MAX_DEVICES];
@@ -387,8 +398,9 @@ extern "C" int bm_linear4(const void* x, int dtype, const uint32_t* payload, con
 
 extern "C" size_t bm_dense_mlp4_workspace_bytes(int32_t T, int32_t intermediate) {
   if (T <= 0 || intermediate <= 0) return 0;
-  // z [T, intermediate], rows of whole 16 bytes, and the per-token gate
-  return align_up(static_cast<size_t>(T) * align_up(intermediate, 8) * 2, 256) + align_up(static_cast<size_t>(T) * 4, 256);
+  // z [T, intermediate], rows of whole 16 bytes, its values that fp16 does not hold, and the per-token gate
+  const size_t z = static_cast<size_t>(T) * align_up(intermediate, 8);
+  return align_up(z * 2, 256) + align_up(z * 4, 256) + align_up(static_cast<size_t>(T) * 4, 256);
 }
 
 extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* gate_payload, const uint16_t* gate_scale, const uint32_t* up_payload,
@@ -407,16 +419,21 @@ extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* g
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int ldz = static_cast<int>(align_up(intermediate, 8));
   void* z = workspace;
-  float* gate = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align_up(static_cast<size_t>(T) * ldz * 2, 256));
+  const size_t nz = static_cast<size_t>(T) * ldz;
+  float* wide = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align_up(nz * 2, 256));
+  float* gate = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(wide) + align_up(nz * 4, 256));
+  if (dtype != BM_F16) wide = nullptr;
   if (token_gate_w && (rc = launch_row_gate(x, dtype, token_gate_w, BM_F16, T, hidden, gate, AFTER_READS, st, true))) return rc;
   Linear4Args a{};
   a.p[0] = gate_payload; a.p[1] = up_payload;
   a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
   a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1; a.beside = token_gate_w != nullptr;
+  a.wide = wide;
   if ((rc = linear4(a, dtype, group, AFTER_READS, st))) return rc;
   Linear4Args d{};
   d.p[0] = down_payload; d.s[0] = reinterpret_cast<const __half*>(down_scale);
   d.x = z; d.residual = residual; d.row_gate = token_gate_w ? gate : nullptr; d.y = y;
   d.T = T; d.K = intermediate; d.N = hidden; d.ldx = ldz; d.ldy = hidden; d.early = 1;
+  d.x_wide = wide;
   return linear4(d, dtype, group, AFTER_READS, st);
 }

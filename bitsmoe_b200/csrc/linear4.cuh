@@ -12,7 +12,9 @@ struct Linear4Args {
   const void* residual;        // [T, N] of y's type, or null
   const float* row_gate;       // factor per token, or null
   void* y;                     // [T, ldy]
-  int T, K, N, ldx, ldy, words, groups;
+  float* wide;                 // GLU with fp16 y: [T, ldy], gets the values that fp16 does not hold (their y is infinite); or null
+  const float* x_wide;         // [T, ldx], such values of x; or null
+  int T, K, N, ldx, ldy, words, groups, group;
   int glu, vec_x, kwarps, splits, row_blocks;
   int early, beside;           // the launch before wrote none of the weights; nothing that this one reads (an AFTER_BESIDE launch behind a `lead` one)
 };
@@ -50,10 +52,40 @@ __device__ __forceinline__ void store_x(void* p, int64_t i, float v) {
   if (XD == BM_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
+// x is the product between the two matrices of an MLP, which may pass fp16's range although the sums over it do not: x is infinite there, and with it
+// every sum of that token.  Sums that are not finite are left out by linear4_finish, and the CTA works them out here, once it is
+// through with everything else, from x's values before their rounding.
+static __device__ __noinline__ void linear4_redo(const Linear4Args& a, int row0, int rows, int tok0, int toks) {
+  for (int o = threadIdx.x; o < rows * toks; o += blockDim.x) {
+    const int token = tok0 + o / rows, row = row0 + o % rows;
+    if (row >= a.N || token >= a.T) continue;
+    const __half *x = static_cast<const __half*>(a.x) + static_cast<int64_t>(token) * a.ldx, *scale = a.s[0] + static_cast<int64_t>(row) * a.groups;
+    const float* wide = a.x_wide + static_cast<int64_t>(token) * a.ldx;
+    const uint32_t* codes = a.p[0] + static_cast<int64_t>(row) * a.words;
+    float sum = 0.f;
+    bool redo = false;
+    for (int k0 = 0; k0 < a.K; k0 += a.group) {
+      float part = 0.f;
+      for (int k = k0; k < min(k0 + a.group, a.K); ++k) {
+        float v = __half2float(x[k]);
+        if (!(fabsf(v) <= 65504.f)) {
+          v = wide[k];
+          redo = true;
+        }
+        part = fmaf(v, static_cast<float>(static_cast<int>(codes[k >> 3] >> (4 * (k & 7)) & 15u) - 8), part);
+      }
+      sum = fmaf(part, __half2float(scale[k0 / a.group]), sum);
+    }
+    // with x finite a sum is not where a scale is not, here as there
+    if (!redo && fabsf(sum) < __int_as_float(0x7f800000)) continue;
+    const float f = a.row_gate ? a.row_gate[token] : 1.f, r = a.residual ? load_x<BM_F16>(a.residual, static_cast<int64_t>(token) * a.N + row) : 0.f;
+    store_x<BM_F16>(a.y, static_cast<int64_t>(token) * a.ldy + row, fmaf(sum, f, r));
+  }
+}
 // Finished sums of one row and up to C tokens: times the tokens' gates, plus the residual, out.  All loads are in flight before the
 // first store (one by one they cost 40 us of a product of 300 tokens, 512 x 2048).
-template <int XD, int C, typename Token>
-__device__ __forceinline__ void linear4_finish(const Linear4Args& a, int row, const float (&v)[C], Token token) {      // token(i) < 0: none
+template <int XD, bool WIDE, int C, typename Token>      // WIDE: a.wide and a.x_wide are looked at
+__device__ __forceinline__ void linear4_finish(const Linear4Args& a, int row, const float (&v)[C], int& left_out, Token token) {      // token(i) < 0: none
   float f[C], r[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {
@@ -70,7 +102,15 @@ __device__ __forceinline__ void linear4_finish(const Linear4Args& a, int row, co
       if (token(i) >= 0) r[i] = load_x<XD>(a.residual, static_cast<int64_t>(token(i)) * a.N + row);
 #pragma unroll
   for (int i = 0; i < C; ++i)
-    if (token(i) >= 0) store_x<XD>(a.y, static_cast<int64_t>(token(i)) * a.ldy + row, fmaf(v[i], f[i], r[i]));
+    if (token(i) >= 0) {
+      if (WIDE && a.x_wide && !(fabsf(v[i]) < __int_as_float(0x7f800000))) {
+        left_out = 1;
+        continue;
+      }
+      const int64_t o = static_cast<int64_t>(token(i)) * a.ldy + row;
+      store_x<XD>(a.y, o, fmaf(v[i], f[i], r[i]));
+      if (WIDE && a.wide && !fits_fp16(v[i])) a.wide[o] = v[i];
+    }
 }
 
 // BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies.

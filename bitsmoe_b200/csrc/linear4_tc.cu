@@ -55,10 +55,12 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   extern __shared__ unsigned char lt_raw[];
   __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_BS], b_empty[LT_BS], a_ready[LT_AS], a_empty[LT_AS], acc_full[LT_ACC], acc_empty[LT_ACC];
   __shared__ uint32_t tmem_slot;
+  __shared__ int left_out;                 // linear4_finish
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char *const b_ring = smem + LT_AS * LT_A_BYTES, *const codes = b_ring + LT_B_RING;
   const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    left_out = 0;
     for (int i = 0; i < LT_PS; ++i) {
       tc::mbar_init(&p_full[i], 1);
       tc::mbar_init(&p_empty[i], LT_CONV_WARPS / 2);
@@ -301,14 +303,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
             const float other = __shfl_xor_sync(0xffffffffu, up ? sum[b][j] : sum[b][j + 1], 16);
             z[j / 2] = up ? silu_mul(other, sum[b][j + 1]) : silu_mul(sum[b][j], other);
           }
-          linear4_finish<XD>(p.a, row, z, [&](int j) { return tok0 + c0 + 2 * j + up < p.a.T && row < p.a.N ? tok0 + c0 + 2 * j + up : -1; });
+          linear4_finish<XD, XD == BM_F16>(p.a, row, z, left_out, [&](int j) { return tok0 + c0 + 2 * j + up < p.a.T && row < p.a.N ? tok0 + c0 + 2 * j + up : -1; });
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = sum[b][8 * h + j];
-            linear4_finish<XD>(p.a, row, v, [&](int j) { return tok0 + c0 + 8 * h + j < p.a.T && row < p.a.N ? tok0 + c0 + 8 * h + j : -1; });
+            linear4_finish<XD, XD == BM_F16>(p.a, row, v, left_out, [&](int j) { return tok0 + c0 + 8 * h + j < p.a.T && row < p.a.N ? tok0 + c0 + 8 * h + j : -1; });
           }
         }
       }
@@ -322,6 +324,12 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   if (p.a.beside) grid_wait();
   tc::fence_before_sync();
   __syncthreads();
+  if (XD == BM_F16 && !GLU && p.a.x_wide && left_out)
+    for (int i = 0; i < mine; ++i) {
+      int row0, tok0, n;
+      tile_of(i, row0, tok0, n);
+      linear4_redo(p.a, row0, LT_ROWS, tok0, min(p.tok_piece, p.a.T - tok0));
+    }
   if (warp == 2) tc::tmem_dealloc(tmem_base, 512);
 }
 

@@ -269,8 +269,9 @@ BM_API int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_
  * host round trips):  y[t] = residual[t] + sum over slots s of topk_w[t, s] * w_down[e] . (silu(gate_e . x[t]) * (up_e . x[t])),
  * e = global_to_local[topk_idx[t, s]] (the id itself when the map is NULL, and then num_routed must equal num_local); slots whose id
  * is not held here add nothing.  w_gate_up [num_local, 2 * intermediate, hidden], gate rows before up rows; w_down [num_local, hidden,
- * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits.  The workspace holds
- * T * k rows of 4 * hidden + 2 * intermediate bytes and the routing lists, whatever share of the slots is held here. */
+ * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits.  The value between the
+ * products is held in `dtype`; where that is fp16 and does not reach, the fp32 value is kept beside it and used.  The workspace holds
+ * T * k rows of 4 * hidden + 6 * intermediate bytes and the routing lists, whatever share of the slots is held here. */
 BM_API size_t bm_dense_experts_workspace_bytes(int32_t T, int32_t k, int32_t num_local, int32_t hidden, int32_t intermediate);
 BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* topk_idx, const float* topk_w, const int32_t* global_to_local,
                                     int32_t num_routed, int32_t T, int32_t k, int32_t num_local, const void* w_gate_up,
@@ -286,7 +287,7 @@ BM_API int bm_linear4(const void* x, int dtype, const uint32_t* payload, const u
                       int32_t group, const void* residual, void* y, void* stream);
 /* SwiGLU MLP with such weights, as bm_dense_mlp_forward: y = f * (silu(x . Wg^T) * (x . Wu^T)) . Wd^T (+ residual), f = 1 or, with
  * token_gate_w (fp16 [hidden]), sigmoid(x . token_gate_w).  gate and up [intermediate, hidden], down [hidden, intermediate]; the value
- * between the products is held in `dtype`. */
+ * between the products is held in `dtype`; where that is fp16 and does not reach, the fp32 value is kept beside it and used. */
 BM_API size_t bm_dense_mlp4_workspace_bytes(int32_t T, int32_t intermediate);
 BM_API int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* gate_payload, const uint16_t* gate_scale,
                                  const uint32_t* up_payload, const uint16_t* up_scale, const uint32_t* down_payload,
