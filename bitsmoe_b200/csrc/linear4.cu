@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   };
   uint32_t w[2][2][L4_BATCH][4];           // [buffer][row][chunk][word]
   float sv[2][2][SPR];                     // lane t: scale of group 4 i + t of the batch
-  grid_launch_dependents();
+  if (!a.lead) grid_launch_dependents();
   if (!a.early && !a.beside) grid_wait();
+  if (a.lead) grid_launch_dependents();
   fetch(w[0], sv[0]);
   if (a.early) grid_wait();
   // ---- x of this CTA's columns, in the order of the products
@@ -427,7 +428,7 @@ extern "C" int bm_dense_mlp4_forward(const void* x, int dtype, const uint32_t* g
   Linear4Args a{};
   a.p[0] = gate_payload; a.p[1] = up_payload;
   a.s[0] = reinterpret_cast<const __half*>(gate_scale); a.s[1] = reinterpret_cast<const __half*>(up_scale);
-  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1; a.beside = token_gate_w != nullptr;
+  a.x = x; a.y = z; a.T = T; a.K = hidden; a.N = intermediate; a.ldx = hidden; a.ldy = ldz; a.glu = 1; a.lead = 1; a.beside = token_gate_w != nullptr;
   a.wide = wide;
   if ((rc = linear4(a, dtype, group, AFTER_READS, st))) return rc;
   Linear4Args d{};

@@ -16,7 +16,10 @@ struct Linear4Args {
   const float* x_wide;         // [T, ldx], such values of x; or null
   int T, K, N, ldx, ldy, words, groups, group;
   int glu, vec_x, kwarps, splits, row_blocks;
-  int early, beside;           // the launch before wrote none of the weights; nothing that this one reads (an AFTER_BESIDE launch behind a `lead` one)
+  // early: fetches weights before it waits.  Everything that may have written them has to be over when it starts, so the launch before is a `lead` one.
+  // lead: lets the next launch start once what came before itself is over, not as soon as it runs.  beside: does not wait before its end,
+  // since the launch before is a lead one that wrote nothing that this one reads.
+  int early, lead, beside;
 };
 
 // Eight codes -> four pairs (code i, code i + 4), i = 0 .. 3, as exact numbers -8 .. 7 of the type.

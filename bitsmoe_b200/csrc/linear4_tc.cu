@@ -86,8 +86,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
-  grid_launch_dependents();
+  if (!p.a.lead) grid_launch_dependents();
   if (!p.a.beside) grid_wait();
+  if (p.a.lead) grid_launch_dependents();
   // tiles of this CTA (neighbours share weight rows), and its slices of their columns: all, or a share that starts with a group
   const int rank = blockIdx.x % p.splits, first = blockIdx.x / p.splits, grid = gridDim.x / p.splits, tiles = p.row_tiles * p.tok_tiles;
   const int mine = tiles > first ? (tiles - first + grid - 1) / grid : 0;

@@ -231,6 +231,33 @@ def test_streams_graphs_and_repeats(tokens):
 
 
 @gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_weights_written_by_the_launch_before(tokens, gated):
+    """Scales of the down matrix that a product of this library has just computed: its launch lets the next ones start early, and the down
+    product fetches weights before it waits.  Every round writes other scales to the same place."""
+    hidden, inter, group = 2048, 1024, 32
+    x, packs, _, tg, res = mlp_case(21, tokens, hidden, inter, group, torch.float16)
+    gen = torch.Generator().manual_seed(22)
+    maker, _ = matrix4(gen, inter // group, 8192, 128)
+    sources = [rnd(gen, hidden, 8192, std=0.02, dtype=torch.float16) for _ in range(3)]
+    tg = tg if gated else None
+    want = []
+    for src in sources:
+        s = linear4(src, *maker)
+        torch.cuda.synchronize()
+        want.append(dense_mlp4(x, packs[0], packs[1], (packs[2][0], s), group, token_gate_weight=tg, residual=res).clone())
+        torch.cuda.synchronize()
+        del s
+    assert not torch.equal(want[0], want[1])
+    for i in range(30):
+        s = linear4(sources[i % 3], *maker)
+        got = dense_mlp4(x, packs[0], packs[1], (packs[2][0], s), group, token_gate_weight=tg, residual=res)
+        assert torch.equal(got, want[i % 3]), i
+        del s, got
+
+
+@gpu
 def test_module_runs_on_the_kernels():
     lin = nn.Linear(192, 80, bias=False, device=DEV).half()
     m = q4.Linear4.from_linear(lin, 64)
