@@ -288,6 +288,56 @@ __global__ void __launch_bounds__(L4_THREADS, l4_ctas(NT)) linear4_kernel(const 
   if (a.beside) grid_wait();
 }
 
+// Any size and alignment: a warp takes a row of the matrix (of each of a gated pair) and eight tokens, element loads, fp32 FMA.  For rows whose columns of
+// x fit no CTA's shared memory and that tiled copies cannot describe.
+constexpr int LA_TOKENS = 8;
+template <int XD, bool GLU>
+__global__ void __launch_bounds__(L4_THREADS) linear4_any_kernel(const __grid_constant__ Linear4Args a) {
+  constexpr int M = GLU ? 2 : 1;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * L4_WARPS + (threadIdx.x >> 5);
+  if (!a.lead) grid_launch_dependents();
+  grid_wait();
+  if (a.lead) grid_launch_dependents();
+  if (row >= a.N) return;
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * LA_TOKENS; n0 < a.T; n0 += static_cast<int64_t>(gridDim.y) * LA_TOKENS) {
+    float acc[M][LA_TOKENS] = {};
+    for (int w = lane; 8 * w < a.K; w += 32) {
+      float part[M][LA_TOKENS] = {};
+      uint32_t code[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) code[m] = __ldg(a.p[m] + static_cast<int64_t>(row) * a.words + w);
+      for (int j = 0; j < 8 && 8 * w + j < a.K; ++j)
+#pragma unroll
+        for (int n = 0; n < LA_TOKENS; ++n) {
+          if (n0 + n >= a.T) break;
+          const int64_t o = (n0 + n) * a.ldx + 8 * w + j;
+          float v = load_x<XD>(a.x, o);
+          if (XD == BM_F16 && a.x_wide && !(fabsf(v) <= 65504.f)) v = a.x_wide[o];
+#pragma unroll
+          for (int m = 0; m < M; ++m) part[m][n] = fmaf(v, static_cast<float>(static_cast<int>(code[m] >> (4 * j) & 15u) - 8), part[m][n]);
+        }
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const float f = __half2float(a.s[m][static_cast<int64_t>(row) * a.groups + 8 * w / a.group]);
+#pragma unroll
+        for (int n = 0; n < LA_TOKENS; ++n) acc[m][n] = fmaf(part[m][n], f, acc[m][n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < LA_TOKENS; ++n) {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[m][n] += __shfl_xor_sync(0xffffffffu, acc[m][n], o);
+      const int64_t t = n0 + n;
+      if (lane != n || t >= a.T) continue;
+      const float v = GLU ? silu_mul(acc[0][n], acc[M - 1][n]) : acc[0][n];
+      store_x<XD>(a.y, t * a.ldy + row, fmaf(v, a.row_gate ? a.row_gate[t] : 1.f, a.residual ? load_x<XD>(a.residual, t * a.N + row) : 0.f));
+      if (XD == BM_F16 && a.wide && !fits_fp16(v)) a.wide[t * a.ldy + row] = v;
+    }
+  }
+}
+
 static size_t l4_smem_bytes(int nt, int K, int splits, bool shared_rows) {
   const int chunks = (K + L4_CHUNK - 1) / L4_CHUNK, cols = nt < 8 ? 8 : nt;
   return static_cast<size_t>((chunks + splits - 1) / splits) * (L4_CHUNK / 8) * nt * 16 + (shared_rows ? static_cast<size_t>(splits) * L4_WARPS * 16 * cols * 4 : 0);
@@ -359,7 +409,14 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
     const int rc = launch_linear4_tc(a, x_dtype, group, after, st);
     if (rc != BM_ERR_UNSUPPORTED) return rc;
   }
-  BM_REQUIRE(fits, BM_ERR_UNSUPPORTED, "linear4: %d rows of %d columns that do not start on 16-byte boundaries", a.T, a.K);
+  if (!fits) {
+    const dim3 any((a.N + L4_WARPS - 1) / L4_WARPS, std::min((a.T + LA_TOKENS - 1) / LA_TOKENS, 65535));
+    auto* kernel = x_dtype == BM_F16 ? (a.glu ? linear4_any_kernel<BM_F16, true> : linear4_any_kernel<BM_F16, false>)
+                                     : (a.glu ? linear4_any_kernel<BM_BF16, true> : linear4_any_kernel<BM_BF16, false>);
+    BM_CUDA(launch_after(after, 1, kernel, any, L4_THREADS, 0, st, a));
+    BM_LAUNCH_CHECK("linear4_any_kernel");
+    return BM_OK;
+  }
   const int grid = std::min(a.row_blocks, std::max(most, 1)) * a.splits;
   const dim3 g(grid, static_cast<unsigned>(passes));
   const size_t smem = l4_smem_bytes(nt, a.K, a.splits, a.kwarps > 1 || a.splits > 1);
