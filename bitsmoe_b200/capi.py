@@ -100,6 +100,8 @@ _SIGS = {
     "bm_dense_mlp4_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
     "bm_dense_mlp4_forward": (C.c_int, [C.c_void_p, C.c_int] + [C.c_void_p] * 7 + [C.c_int32] * 4 + [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                                                                                    C.c_void_p]),
+    "bm_dense_status": (C.c_int, [C.c_void_p]),
+    "bm_dense_set_wait_limit": (C.c_int, [C.c_int32]),
     "bm_ep_flag_bytes": (C.c_size_t, []),
     "bm_ep_barrier": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "bm_ep_push": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),

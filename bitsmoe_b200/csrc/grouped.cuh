@@ -65,6 +65,13 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 // Whether rounding v to fp16 leaves a number (65520 is half way from the largest one to the next power of two).
 __device__ __forceinline__ bool fits_fp16(float v) { return fabsf(v) < 65520.f; }
 
+// Where the kernels of the dense products report a wait that gave up, and how long one waits (0: as if one had given up at the start).
+struct DenseGuard {
+  int* status;
+  uint64_t limit_ns;
+};
+int dense_guard(DenseGuard* g);      // of the current device
+
 // BM_ERR_UNSUPPORTED, with nothing launched, when a shape or pointer does not suit tiled copies (grouped_tc.cu).
 int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st);
 // Whether rows picked by an index are brought into expert order before the products.

@@ -12,7 +12,8 @@
 //               shared memory, so that a thread stores 16 bytes of a row of y.  With a gated pair the accumulator's lanes alternate between
 //               16 gate rows and the 16 up rows that belong to them, so that a thread holds both sums of an output.
 // The accumulator alternates between two halves of tensor memory.  Items are handed out round robin; which expert an item belongs
-// to every CTA works out from the offsets, so that the host never reads them.  Waits are bounded.
+// to every CTA works out from the offsets, so that the host never reads them.  Waits are bounded; one that gives up raises the
+// status word, and the pair leaves once its copies and products are done.
 //
 // Measured (bf16, K 2048, N 1536): 128 groups in order of 1 row 121 us (HBM floor 123), 128 rows 151, 512 rows 315 (1.3 PFLOP/s); one group of 65536 rows 290
 // (1.42 PFLOP/s, what the library product reaches under the power limit).  Few rows are bound by HBM, many by the tensor pipe at its
@@ -44,6 +45,7 @@ struct GcParams {
   const int32_t* index;
   void* y;
   float* wide;
+  DenseGuard guard;
   int x_rows, rows, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
   SlotArgs slots;
 };
@@ -140,7 +142,9 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 template <bool GLU, bool GATHER, bool F32, bool BF16>
 __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_constant__ GcParams p) {
   extern __shared__ unsigned char gc_raw[];
-  __shared__ __align__(8) uint64_t full[GC_MAX_STAGES], empty[GC_MAX_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[GC_MAX_STAGES], empty[GC_MAX_STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ int gave_up;                  // a wait of either CTA ran out
+  __shared__ int issued[4];                // stages that either CTA's producers (2 rank, 2 rank + 1) have issued
   __shared__ uint32_t tmem_slot;
   __shared__ int longest;
   __shared__ int4 rows4[32];
@@ -155,6 +159,8 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
+    gave_up = p.guard.limit_ns == 0;
+    tc::mbar_init(&drained, 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
       tc::mbar_init(&acc_empty[i], 2 * GC_EPI_WARPS);
@@ -214,17 +220,21 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   const int slice = a_bytes + longest / 2 * GC_K * 2, sub = slice <= GC_RING / 32 ? 4 : slice <= GC_RING / 10 ? 2 : 1;
   const int stages = min(GC_RING / (slice * sub), GC_MAX_STAGES);
   bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_wait_limit(bar, parity, p.guard.limit_ns); };
+  auto to_both = [&](int* what, int v) {
+    for (uint32_t r = 0; r < 2; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_map(tc::smem_u32(what), r)), "r"(v) : "memory");
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ weight rows
     uint32_t st = 0, ph = 0;
-    int e = 0;
+    int e = 0, n = 0;
     for (int item = pair; item < items && ok; item += pairs) {
       const GcItem it = gc_item(tab, item, e);
       const uint32_t bytes = 2 * (a_bytes + (it.n() >> 1) * GC_K * 2);      // of both CTAs' slices
       const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2);
       for (int k0 = 0; k0 < p.slices; k0 += sub) {
-        if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
+        if (!(ok = wait(&empty[st], ph ^ 1))) break;
         if (tc::elect_one()) {
           const int cnt = min(sub, p.slices - k0);
           const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
@@ -244,13 +254,15 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
           }
         }
         __syncwarp();
+        ++n;
         if (++st == stages) { st = 0; ph ^= 1; }
       }
     }
+    if (lane == 0) to_both(&issued[2 * rank + (warp != 0)], n);
   } else if (warp == 3) {
     // ------------------------------------------------------------------ rows of x
     uint32_t st = 0, ph = 0;
-    int e = 0;
+    int e = 0, n = 0;
     for (int item = pair; item < items && ok; item += pairs) {
       const GcItem it = gc_item(tab, item, e);
       const int half = it.n() >> 1, first = it.row0 + static_cast<int>(rank) * half;
@@ -267,7 +279,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
         __syncwarp();
       }
       for (int k0 = 0; k0 < p.slices; k0 += sub) {
-        if (!(ok = tc::mbar_wait(&empty[st], ph ^ 1))) break;
+        if (!(ok = wait(&empty[st], ph ^ 1))) break;
         if (tc::elect_one()) {
           const int cnt = min(sub, p.slices - k0);
           const uint32_t bar = tc::cluster_map(tc::smem_u32(&full[st]), 0);
@@ -285,9 +297,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
           }
         }
         __syncwarp();
+        ++n;
         if (++st == stages) { st = 0; ph ^= 1; }
       }
     }
+    if (lane == 0) to_both(&issued[2 * rank + (warp != 0)], n);
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------------ MMA issue
     uint32_t st = 0, ph = 0, ti = 0;
@@ -295,10 +309,10 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
       const GcItem it = gc_item(tab, item, e);
       const uint32_t ab = ti & 1u, idesc = BF16 ? tc::idesc_bf16(256, it.n()) : tc::idesc_f16(256, it.n()), parts = it.parts(), apart = GC_ROWS / parts;
-      if (ti >= 2 && !(ok = tc::mbar_wait_cluster(&acc_empty[ab], ((ti >> 1) - 1) & 1))) break;    // read out two items ago
+      if (ti >= 2 && !(ok = tc::mbar_wait_limit<true>(&acc_empty[ab], ((ti >> 1) - 1) & 1, p.guard.limit_ns))) break;    // read out two items ago
       tc::fence_after_sync();
       for (int k0 = 0; k0 < p.slices; k0 += sub) {
-        if (!(ok = tc::mbar_wait(&full[st], ph))) break;
+        if (!(ok = wait(&full[st], ph))) break;
         tc::fence_after_sync();
         if (tc::elect_one()) {
           const int cnt = min(sub, p.slices - k0);
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     for (int item = pair; item < items && ok; item += pairs, ++ti) {
       const GcItem it = gc_item(tab, item, e);
       const uint32_t ab = ti & 1u;
-      if (!(ok = tc::mbar_wait(&acc_full[ab], (ti >> 1) & 1))) break;
+      if (!(ok = wait(&acc_full[ab], (ti >> 1) & 1))) break;
       tc::fence_after_sync();
       const uint32_t acc = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + ab * GC_ROWS;
       const int col0 = (it.block * 2 + static_cast<int>(rank)) * quarters * (QUARTER / 2) + WIDE * q, parts = it.parts();
@@ -415,10 +429,41 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       if (lane == 0) tc::mbar_arrive_release_cluster(tc::cluster_map(tc::smem_u32(&acc_empty[ab]), 0));
     }
   }
+  if (!ok && lane == 0) to_both(&gave_up, 1);
   tc::fence_before_sync();
   __syncthreads();
   tc::cluster_arrive();
-  tc::cluster_wait();                          // nothing of the other CTA reaches into this one any more
+  tc::cluster_wait();                          // nothing of the other CTA reaches into this one any more, but for copies and products where a wait gave up
+  if (gave_up) {
+    // Stages that one producer has issued and another has not would never be full: the others' bytes are made up, for at most a ring of
+    // stages, since nobody is a ring ahead of a stage that is not full.  Then the last copies into every stage are waited for, and the products.
+    const int upto = max(max(issued[0], issued[1]), max(issued[2], issued[3]));
+    if ((warp == 0 || warp == 3) && tc::elect_one()) {
+      int k = 0, e = 0;
+      for (int item = pair; item < items && k < upto; item += pairs) {
+        const GcItem it = gc_item(tab, item, e);
+        const uint32_t of_x = (it.n() >> 1) * GC_K * 2;
+        for (int k0 = 0; k0 < p.slices && k < upto; k0 += sub, ++k) {
+          if (k < issued[2 * rank + (warp != 0)]) continue;
+          const int cnt = min(sub, p.slices - k0);
+          if (warp == 0 && rank == 0) tc::mbar_expect_tx(&full[k % stages], cnt * 2 * (a_bytes + of_x));
+          tc::mbar_complete_tx(tc::cluster_map(tc::smem_u32(&full[k % stages]), 0), cnt * (warp == 0 ? a_bytes : of_x));
+        }
+      }
+    }
+    __syncwarp();
+    if (warp == 0 && rank == 0)
+      for (int k = max(0, upto - stages); k < upto; ++k) tc::mbar_wait(&full[k % stages], (k / stages) & 1);
+    if (warp == 1) {
+      if (rank == 0 && tc::elect_one()) tc::mma_commit_pair(&drained);
+      __syncwarp();
+      tc::mbar_wait(&drained, 0);
+    }
+    if (threadIdx.x == 0) atomicExch(p.guard.status, BM_ERR_TIMEOUT);
+    __syncthreads();
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
   if (warp == 2) tc::tmem_dealloc_pair(tmem_base, 512);
 }
 
@@ -468,6 +513,8 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   int dev = -1;
   BM_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= MAX_DEVICES) return BM_ERR_UNSUPPORTED;
+  const int rc = dense_guard(&p.guard);
+  if (rc) return rc;
   if (!once.is_done(dev)) {
     for (auto& k : GC_KERNELS) BM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, gc_smem_bytes(GC_MAX_E)));
     BM_CUDA(cudaDeviceGetAttribute(&grids[dev], cudaDevAttrMultiProcessorCount, dev));

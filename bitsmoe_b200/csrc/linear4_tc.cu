@@ -12,7 +12,8 @@
 //   warps 4-11   epilogue: lane quarter, every other block of 16 tokens
 // Where there are few tiles, clusters of CTAs share a tile's columns and add their sums up in the first one's shared memory, in order.
 // With a gated pair the rows alternate between 16 gate rows and the 16 up rows that belong to them; lanes l and l + 16 exchange every
-// other token's sums at the end.  Waits are bounded.
+// other token's sums at the end.  Waits are bounded; one that gives up raises the status word, and the CTA leaves once its copies and
+// products are done.
 //
 // Measured (bf16, groups of 128): 4096 x 4096 at 64 / 256 / 1024 tokens 19 / 27 / 76 us (0.11 / 0.31 / 0.45 PFLOP/s).  A slice of 64 columns costs 0.45 us of waits, four
 // products and commits whatever the tile's width, a launch 8 to 10 us of start, first data, exchange and end.
@@ -37,6 +38,7 @@ constexpr int LT_SMEM = LT_PS * LT_P_BYTES + LT_AS * LT_A_BYTES + LT_B_RING + 10
 struct LtParams {
   CUtensorMap x, x8, p[2];     // x: 32 tokens or 8
   Linear4Args a;
+  DenseGuard guard;
   int splits, slices, row_tiles, tok_tiles, tok_piece, per_group;      // splits: CTAs that share a tile's columns; per_group: products of K = 16
 };
 
@@ -53,14 +55,17 @@ __device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
 template <int XD, bool GLU>
 __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_constant__ LtParams p) {
   extern __shared__ unsigned char lt_raw[];
-  __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_BS], b_empty[LT_BS], a_ready[LT_AS], a_empty[LT_AS], acc_full[LT_ACC], acc_empty[LT_ACC];
+  __shared__ __align__(8) uint64_t p_full[LT_PS], p_empty[LT_PS], b_full[LT_BS], b_empty[LT_BS], a_ready[LT_AS], a_empty[LT_AS], acc_full[LT_ACC], acc_empty[LT_ACC], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int left_out;                 // linear4_finish
+  __shared__ int gave_up;                  // a wait of this CTA ran out
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char *const b_ring = smem + LT_AS * LT_A_BYTES, *const codes = b_ring + LT_B_RING;
   const int warp = tc::warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     left_out = 0;
+    gave_up = p.guard.limit_ns == 0;
+    tc::mbar_init(&drained, 1);
     for (int i = 0; i < LT_PS; ++i) {
       tc::mbar_init(&p_full[i], 1);
       tc::mbar_init(&p_empty[i], LT_CONV_WARPS / 2);
@@ -102,6 +107,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
   };
   const int b_bytes = p.tok_piece * LT_K * 2, b_stages = min(LT_B_RING / b_bytes, LT_BS);
   bool ok = true;
+  int issued = 0;                          // stages of copies under way or done (warps 0 and 3)
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_wait_limit(bar, parity, p.guard.limit_ns); };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ codes, as far ahead as there are slots
@@ -110,7 +117,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       int row0, tok0, n;
       tile_of(i, row0, tok0, n);
       for (int k = k_first; k < k_end; ++k) {
-        if (!(ok = tc::mbar_wait(&p_empty[slot], ph))) break;
+        if (!(ok = wait(&p_empty[slot], ph))) break;
         if (tc::elect_one()) {
           unsigned char* to = codes + slot * LT_P_BYTES;
           tc::mbar_expect_tx(&p_full[slot], LT_P_BYTES);
@@ -118,6 +125,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
           lt_load_2d(to + LT_P_BYTES / 2, &p.p[GLU], k * (LT_K / 2), GLU ? row0 : row0 + LT_ROWS / 2, &p_full[slot]);
         }
         __syncwarp();
+        ++issued;
         if (++slot == LT_PS) { slot = 0; ph ^= 1; }
       }
     }
@@ -128,7 +136,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       int row0, tok0, n;
       tile_of(i, row0, tok0, n);
       for (int k = k_first; k < k_end; ++k) {
-        if (!(ok = tc::mbar_wait(&b_empty[st], ph))) break;
+        if (!(ok = wait(&b_empty[st], ph))) break;
         if (tc::elect_one()) {
           unsigned char* to = b_ring + st * b_bytes;
           tc::mbar_expect_tx(&b_full[st], n * LT_K * 2);
@@ -137,6 +145,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
           for (; r < n; r += 8) lt_load_2d(to + r * (LT_K * 2), &p.x8, k * LT_K, tok0 + r, &b_full[st]);
         }
         __syncwarp();
+        ++issued;
         if (++st == b_stages) { st = 0; ph ^= 1; }
       }
     }
@@ -152,7 +161,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       int in_group = 0;
       for (int k = 0; k < slices && ok; ++k, ++s) {
         const int st = s % LT_AS;
-        if (!(ok = tc::mbar_wait(&b_full[bs], b_ph) && tc::mbar_wait(&a_ready[st], (s / LT_AS) & 1))) break;
+        if (!(ok = wait(&b_full[bs], b_ph) && wait(&a_ready[st], (s / LT_AS) & 1))) break;
         tc::fence_after_sync();
         const uint64_t ad = lt_desc(tc::smem_u32(smem + st * LT_A_BYTES)), bd = lt_desc(tc::smem_u32(b_ring + bs * b_bytes));
         // the slice's products of one group at a time: four, or two and two
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
           if (h == 1 && !two) break;
           const uint32_t buf = acc % LT_ACC, d = tmem_base + buf * LT_TOK;
           if (in_group == 0) {
-            if (acc >= LT_ACC && !(ok = tc::mbar_wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
+            if (acc >= LT_ACC && !(ok = wait(&acc_empty[buf], (acc / LT_ACC - 1) & 1))) break;
             tc::fence_after_sync();
           }
           const bool last = two || in_group + 4 == p.per_group || end;
@@ -191,7 +200,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
     const int grp = (warp - LT_CONV0) / (LT_CONV_WARPS / 2), i = threadIdx.x - 32 * LT_CONV0 - grp * (16 * LT_CONV_WARPS);
     for (int s = grp; s < total; s += 2) {
       const int slot = s % LT_PS, st = s % LT_AS;
-      if (!(ok = tc::mbar_wait(&p_full[slot], (s / LT_PS) & 1))) break;
+      if (!(ok = wait(&p_full[slot], (s / LT_PS) & 1))) break;
       uint4 w[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -200,7 +209,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
         const int src = GLU ? ((m & 16) ? LT_ROWS / 2 : 0) + 16 * (m >> 5) + (m & 15) : m;
         w[u] = *reinterpret_cast<const uint4*>(codes + slot * LT_P_BYTES + src * (LT_K / 2) + (piece & 1) * 16);
       }
-      if (s >= LT_AS && !(ok = tc::mbar_wait(&a_empty[st], (s / LT_AS - 1) & 1))) break;
+      if (s >= LT_AS && !(ok = wait(&a_empty[st], (s / LT_AS - 1) & 1))) break;
       unsigned char* const to = smem + st * LT_A_BYTES;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -248,7 +257,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
         for (int j = 0; j < 4; ++j) {
           if (g0 + j >= g_end) break;
           const uint32_t buf = acc % LT_ACC;
-          if (!(ok = tc::mbar_wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
+          if (!(ok = wait(&acc_full[buf], (acc / LT_ACC) & 1))) break;
           tc::fence_after_sync();
           const uint32_t at = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + buf * LT_TOK;
           const float f = __half2float(__ushort_as_half(static_cast<unsigned short>(now[j])));
@@ -322,9 +331,24 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear4_tc_kernel(const __grid_
       tc::cluster_arrive();
       tc::cluster_wait();
     }
+  if (!ok && lane == 0) gave_up = 1;
   if (p.a.beside) grid_wait();
   tc::fence_before_sync();
   __syncthreads();
+  if (gave_up) {
+    // nothing may be under way when the CTA leaves: the last copies into every slot and stage, and the products
+    if (warp == 0)
+      for (int k = max(0, issued - LT_PS); k < issued; ++k) tc::mbar_wait(&p_full[k % LT_PS], (k / LT_PS) & 1);
+    if (warp == 3)
+      for (int k = max(0, issued - b_stages); k < issued; ++k) tc::mbar_wait(&b_full[k % b_stages], (k / b_stages) & 1);
+    if (warp == 1) {
+      if (tc::elect_one()) tc::mma_commit(&drained);
+      __syncwarp();
+      tc::mbar_wait(&drained, 0);
+    }
+    if (threadIdx.x == 0) atomicExch(p.guard.status, BM_ERR_TIMEOUT);
+    __syncthreads();
+  }
   if (XD == BM_F16 && !GLU && p.a.x_wide && left_out)
     for (int i = 0; i < mine; ++i) {
       int row0, tok0, n;
@@ -372,6 +396,8 @@ int launch_linear4_tc(const Linear4Args& args, int x_dtype, int group, LaunchAft
   int dev = -1;
   BM_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= MAX_DEVICES) return BM_ERR_UNSUPPORTED;
+  const int rc = dense_guard(&p.guard);
+  if (rc) return rc;
   if (!once.is_done(dev)) {
     for (auto* kernel : {linear4_tc_kernel<BM_F16, false>, linear4_tc_kernel<BM_F16, true>, linear4_tc_kernel<BM_BF16, false>, linear4_tc_kernel<BM_BF16, true>})
       BM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM));

@@ -23,6 +23,10 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// What a copy of `bytes` bytes does to the barrier at `mapped` (shared::cluster address) once it is there.
+__device__ __forceinline__ void mbar_complete_tx(uint32_t mapped, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(mapped), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -50,18 +54,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
   }
   return false;
 }
-// The same for what threads of another CTA of the cluster have published with a release at cluster scope.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns = WAIT_LIMIT_NS) {
-  const uint32_t addr = smem_u32(bar);
+// The same with a limit that a caller sets; 0: a wait that is not over at once gives up.  CLUSTER: for what threads of another CTA of the
+// cluster have published with a release at cluster scope.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait_limit(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  const uint32_t addr = smem_u32(bar), suspend = limit_ns == 0 ? 0u : 20000u;
   uint64_t t0 = 0;
   for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity), "r"(20000u)
-        : "memory");
+    if (CLUSTER)
+      asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                   : "=r"(done)
+                   : "r"(addr), "r"(parity), "r"(suspend)
+                   : "memory");
+    else
+      asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                   : "=r"(done)
+                   : "r"(addr), "r"(parity), "r"(suspend)
+                   : "memory");
     if (done) return true;
+    if (limit_ns == 0) return false;
     if ((i & 15u) == 15u) {
       const uint64_t now = global_ns();
       if (t0 == 0) t0 = now;

@@ -335,3 +335,11 @@ def dense_mlp4(x: torch.Tensor, gate: Tuple[torch.Tensor, torch.Tensor], up: Tup
     if not x.is_cuda:
         raise RuntimeError("dense_mlp4 requires CUDA tensors; there is no CPU path")
     return capi.host().dense_mlp4(x, *gate, *up, *down, group_size, None if token_gate_weight is None else token_gate_weight.reshape(-1), residual)
+
+
+def check_dense_status(device: Optional[torch.device] = None) -> None:
+    """Synchronises the current stream of ``device`` and raises when a kernel of ``grouped_linear``, ``dense_experts``, ``linear4`` or
+    ``dense_mlp4`` has given up a bounded wait there since the last call, as ``PackedLayer.check_status`` does for a layer."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(device):
+        capi.check(capi.lib().bm_dense_status(capi.stream_ptr(device)))

@@ -278,6 +278,14 @@ BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* top
                                     const void* w_down, int32_t hidden, int32_t intermediate, const void* residual, void* y,
                                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* The kernels of these products and of those with 4-bit weights wait within limits.  bm_dense_status synchronises `stream` and reports whether one
+ * of them has given up a wait on the current device since the last call (BM_ERR_TIMEOUT; the outputs of that call are undefined), as
+ * bm_layer_status does for a layer.  bm_dense_set_wait_limit: longest time of a wait from the next call on, 0 .. 2000000 us (the
+ * default); with 0 a kernel starts as if a wait had run out: waits that are not over at once give up, and it leaves with its copies and products
+ * done.  It is how that way out is tested. */
+BM_API int bm_dense_status(void* stream);
+BM_API int bm_dense_set_wait_limit(int32_t limit_us);
+
 /* ---- products with 4-bit weights ------------------------------------------
  * y[t][n] = sum_k x[t][k] * scale[n][k / group] * (code[n][k] - 8) (+ residual): x [T, K], residual (may be NULL) and y [T, N] of
  * `dtype` (fp16 or bf16).  payload uint32 [N, 4 * ceil(K / 32)], 16-byte aligned: the code of column 8 j + i in bits 4 i .. 4 i + 3 of
