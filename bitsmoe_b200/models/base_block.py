@@ -43,6 +43,7 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         self._super_expert_items: List[Tuple[int, nn.Module]] = []
         self._super_weights: Optional[Tuple[torch.Tensor, torch.Tensor]] = None     # gate and up rows [E, 2I, H], down [E, H, I]
         self._super_global_to_local: Optional[torch.Tensor] = None
+        self._super_map_of: Optional[tuple] = None          # (device, entries) of that map
         self._packed_expert_count = 0
         self._packed_intermediate_size = 0
         self._packed_global_to_local: Optional[torch.Tensor] = None
@@ -144,9 +145,11 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
         supers = torch.full((self.num_experts,), -1, dtype=torch.int32)
         for local, (idx, _) in enumerate(super_items):
             supers[idx] = local
-        self._super_global_to_local = supers.to(device) if super_items else None
+        # map and stack outlive the cache where they still hold: a captured graph of the un-quantised experts reads them
         if not super_items:
-            self._super_weights = None           # otherwise the parameters are its slices as long as they live where they do
+            self._super_global_to_local = self._super_weights = None
+        elif self._super_global_to_local is None or self._super_map_of != (device, supers.tolist()):
+            self._super_global_to_local, self._super_map_of = supers.to(device), (device, supers.tolist())
         self._identity_map = self._packed_expert_count == self.num_experts and not super_items
         modules = [m for _, m in packed_items]
         for tag in _TAGS:

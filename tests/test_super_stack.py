@@ -79,11 +79,12 @@ def test_loading_weights_keeps_the_stack():
     """What is loaded goes into the slices: the stack that a captured graph reads stays the one in use."""
     blk = host_block({1: mlp(1), 4: mlp(2)})
     gu, dn = blk._stacked_super_weights()
+    ids = blk._super_global_to_local
     doubled = {k: v * 2 if "experts" in k else v for k, v in blk.state_dict().items()}
     blk.load_state_dict(doubled)
     blk._ensure_runtime_cache(torch.device("cpu"))
     again = blk._stacked_super_weights()
-    assert again[0] is gu and again[1] is dn and torch.equal(gu[1, :INTER], doubled["experts.4.gate_proj.weight"])
+    assert blk._super_global_to_local is ids and again[0] is gu and again[1] is dn and torch.equal(gu[1, :INTER], doubled["experts.4.gate_proj.weight"])
     blk.set_expert(4, mlp(3), packed=False)                  # another module: another stack
     blk._ensure_runtime_cache(torch.device("cpu"))
     assert blk._stacked_super_weights()[0] is not gu
