@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(256) slot_places_kernel(const SlotArgs a) {
   grid_launch_dependents();
   grid_wait();
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < a.slots) a.pos[i] = slot_place(a, i);
+  const int2 r = slot_range(a);
+  if (i >= r.x && i < r.y) a.pos[i] = slot_place(a, i);
 }
 
 bool grouped_gathers(int expected, int E, int K) { return K % 8 == 0 && expected / E >= GATHER_ROWS; }
@@ -175,7 +176,7 @@ struct CombineArgs {
   const float* topk_w;
   const void* residual;
   void* y;
-  int k, H, vec;               // vec: H % 4 == 0, y and the residual on 8-byte boundaries
+  int T, k, H, vec;            // vec: H % 4 == 0, y and the residual on 8-byte boundaries
   // fp16: what the down product was made of
   SlotArgs slots;
   const void *z, *w_down;      // [rows, I], [E, H, I]
@@ -206,72 +207,162 @@ __device__ __forceinline__ float4 load4(const void* p, int64_t i) {
 }
 template <int D>
 __global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const CombineArgs a) {
-  const int t = blockIdx.x, h = (blockIdx.y * EC_THREADS + threadIdx.x) * 4;
+  const int h = (blockIdx.y * EC_THREADS + threadIdx.x) * 4;
   grid_launch_dependents();
   grid_wait();
   if (h >= a.H) return;
-  const int64_t o = static_cast<int64_t>(t) * a.H + h;
-  const int n = min(4, a.H - h);
-  float v[4] = {};
-  if (a.residual) {
-    if (a.vec) *reinterpret_cast<float4*>(v) = load4<D>(a.residual, o);
-    else
-      for (int j = 0; j < n; ++j) v[j] = load16<D>(a.residual, o + j);
-  }
-  for (int s0 = 0; s0 < a.k; s0 += 8) {
-    float4 d[8];
-    float w[8];
+  const int2 tokens = a.slots.window ? make_int2(__ldcg(a.slots.window), __ldcg(a.slots.window + 1)) : make_int2(0, a.T);
+  for (int t = tokens.x + blockIdx.x; t < tokens.y; t += gridDim.x) {
+    const int64_t o = static_cast<int64_t>(t) * a.H + h;
+    const int n = min(4, a.H - h);
+    float v[4] = {};
+    if (a.residual) {
+      if (a.vec) *reinterpret_cast<float4*>(v) = load4<D>(a.residual, o);
+      else
+        for (int j = 0; j < n; ++j) v[j] = load16<D>(a.residual, o + j);
+    }
+    for (int s0 = 0; s0 < a.k; s0 += 8) {
+      float4 d[8];
+      float w[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int at = s0 + u < a.k ? __ldg(a.pos + static_cast<int64_t>(t) * a.k + s0 + u) : -1;
-      w[u] = at >= 0 ? __ldg(a.topk_w + static_cast<int64_t>(t) * a.k + s0 + u) : 0.f;
-      d[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (at >= 0) {
-        const float* src = a.d + static_cast<int64_t>(at) * a.H + h;
-        if (a.vec) d[u] = __ldcs(reinterpret_cast<const float4*>(src));
-        else {
-          d[u].x = src[0];
-          if (n > 1) d[u].y = src[1];
-          if (n > 2) d[u].z = src[2];
-          if (n > 3) d[u].w = src[3];
+      for (int u = 0; u < 8; ++u) {
+        const int at = s0 + u < a.k ? __ldg(a.pos + static_cast<int64_t>(t) * a.k + s0 + u) : -1;
+        w[u] = at >= 0 ? __ldg(a.topk_w + static_cast<int64_t>(t) * a.k + s0 + u) : 0.f;
+        d[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at >= 0) {
+          const float* src = a.d + static_cast<int64_t>(at) * a.H + h;
+          if (a.vec) d[u] = __ldcs(reinterpret_cast<const float4*>(src));
+          else {
+            d[u].x = src[0];
+            if (n > 1) d[u].y = src[1];
+            if (n > 2) d[u].z = src[2];
+            if (n > 3) d[u].w = src[3];
+          }
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      v[0] = fmaf(w[u], d[u].x, v[0]);
-      v[1] = fmaf(w[u], d[u].y, v[1]);
-      v[2] = fmaf(w[u], d[u].z, v[2]);
-      v[3] = fmaf(w[u], d[u].w, v[3]);
-    }
-  }
-  if (D == BM_F16 && !(fabsf((v[0] + v[1]) + (v[2] + v[3])) < __int_as_float(0x7f800000)))
-    // once more, slot by slot, with the rows of d that are not finite worked out anew
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      float sum = a.residual ? load16<D>(a.residual, o + j) : 0.f;
-#pragma unroll 1
-      for (int s = 0; s < a.k; ++s) {
-        const int slot = t * a.k + s, at = a.pos[slot];
-        if (at < 0) continue;
-        float d = a.d[static_cast<int64_t>(at) * a.H + h + j];
-        if (!(fabsf(d) < __int_as_float(0x7f800000))) d = wide_down(a, slot, at, h + j);
-        sum = fmaf(a.topk_w[slot], d, sum);
+      for (int u = 0; u < 8; ++u) {
+        v[0] = fmaf(w[u], d[u].x, v[0]);
+        v[1] = fmaf(w[u], d[u].y, v[1]);
+        v[2] = fmaf(w[u], d[u].z, v[2]);
+        v[3] = fmaf(w[u], d[u].w, v[3]);
       }
-      v[0] = j == 0 ? sum : v[0]; v[1] = j == 1 ? sum : v[1]; v[2] = j == 2 ? sum : v[2]; v[3] = j == 3 ? sum : v[3];
     }
-  uint16_t out[4];
+    if (D == BM_F16 && !(fabsf((v[0] + v[1]) + (v[2] + v[3])) < __int_as_float(0x7f800000)))
+      // once more, slot by slot, with the rows of d that are not finite worked out anew
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        float sum = a.residual ? load16<D>(a.residual, o + j) : 0.f;
+#pragma unroll 1
+        for (int s = 0; s < a.k; ++s) {
+          const int slot = t * a.k + s, at = a.pos[slot];
+          if (at < 0) continue;
+          float d = a.d[static_cast<int64_t>(at) * a.H + h + j];
+          if (!(fabsf(d) < __int_as_float(0x7f800000))) d = wide_down(a, slot, at, h + j);
+          sum = fmaf(a.topk_w[slot], d, sum);
+        }
+        v[0] = j == 0 ? sum : v[0]; v[1] = j == 1 ? sum : v[1]; v[2] = j == 2 ? sum : v[2]; v[3] = j == 3 ? sum : v[3];
+      }
+    uint16_t out[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] = D == BM_F16 ? __half_as_ushort(__float2half_rn(v[j])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
-  if (a.vec) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + o) = make_uint2(out[0] | out[1] << 16, out[2] | out[3] << 16);
-  else
-    for (int j = 0; j < n; ++j) static_cast<uint16_t*>(a.y)[o + j] = out[j];
+    for (int j = 0; j < 4; ++j) out[j] = D == BM_F16 ? __half_as_ushort(__float2half_rn(v[j])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
+    if (a.vec) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + o) = make_uint2(out[0] | out[1] << 16, out[2] | out[3] << 16);
+    else
+      for (int j = 0; j < n; ++j) static_cast<uint16_t*>(a.y)[o + j] = out[j];
+  }
+}
+
+// Rows of scratch.  A short batch has one for every assignment, since all may name experts held here.  Where few are held most would stay empty: of 32768
+// tokens of ten experts, three of 512 held (2048 hidden, 512), 3.7 GB for the 20 MB that are used.  Beyond 256 MB a token therefore has
+// min(k, experts held) rows (slots that name the same expert share one), and beyond 1 GB, or four times the weights where that is more, the batch goes
+// through in windows of tokens: a window takes all that is left when its rows fit, which the device finds out, and else as many tokens as fit
+// for certain.  There are as many windows as that may need, the others find nothing to do, at 20 to 25 us each.  4096 / 16384 / 32768
+// tokens of that layer took 61 / 141 / 242 us and 0.4 / 1.5 / 3.0 GB with a row for every assignment, and take 68 / 155 / 296 and 0.15 / 0.6 / 1.15
+// (bf16, the output among them).
+struct DenseRows {
+  int64_t rows;
+  int per, step;               // of a token at most; tokens that fit for certain
+  DenseRows(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    const double row = 4.0 * H + 6.0 * I, room = std::max(double(1ll << 30), 24.0 * E * H * I);
+    per = static_cast<int>(T * k * row <= double(256ll << 20) ? k : std::min(k, E));
+    const int64_t fit = static_cast<int64_t>(std::min(room / row, 1e9));
+    rows = std::min(T * per, std::max<int64_t>(fit, per));
+    step = static_cast<int>(rows / per);
+  }
+};
+
+// Slots that name an expert of an earlier slot of their token are taken out of the selection: a warp per token.
+__global__ void __launch_bounds__(256) experts_distinct_kernel(const SlotArgs a, int T, int32_t* idx) {
+  grid_launch_dependents();
+  grid_wait();
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= T) return;
+  const int e = lane < a.k ? slot_expert(a, t * a.k + lane) : -1;
+  const unsigned same = __match_any_sync(0xffffffffu, e);
+  if (lane < a.k) idx[static_cast<int64_t>(t) * a.k + lane] = e >= 0 && __ffs(same) - 1 == lane ? a.topk_idx[t * a.k + lane] : -1;
+}
+
+struct WindowArgs {
+  const int32_t *tok, *off;    // all rows: token of each, offsets [E + 1]
+  int32_t *wtok, *woff;        // the window's
+  int32_t* bounds;             // [2] its tokens from, to; of the window before on entry
+  int T, E, rows, step, first; // rows there are; tokens that fit for certain
+};
+// One CTA: a thread per expert finds the window's part of its list (tokens ascend in it), warps copy it.
+constexpr int EW_THREADS = 1024;
+__global__ void __launch_bounds__(EW_THREADS) experts_window_kernel(const WindowArgs a) {
+  __shared__ int from[EW_THREADS], sums[EW_THREADS / 32], start[EW_THREADS + 1];
+  grid_launch_dependents();
+  grid_wait();
+  const int e = threadIdx.x, lane = e & 31, warp = e >> 5, t0 = a.first ? 0 : a.bounds[1];
+  const int begin = e < a.E ? a.off[e] : 0, end = e < a.E ? a.off[e + 1] : 0;
+  auto first_of = [&](int t) {
+    int lo = begin, hi = end;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.tok[mid] < t) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo;
+  };
+  auto inclusive = [&](int v) {      // over the block
+    __syncthreads();
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += n;
+    }
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) v += sums[w];
+    return v;
+  };
+  const int lo = first_of(t0);
+  from[e] = lo;
+  start[e + 1] = inclusive(end - lo);
+  __syncthreads();
+  const int t1 = start[EW_THREADS] <= a.rows ? a.T : min(a.T, t0 + a.step);
+  const int n = first_of(t1) - lo, upto = inclusive(n);
+  start[e + 1] = upto;
+  if (e == 0) {
+    start[0] = 0;
+    a.woff[0] = 0;
+    a.bounds[0] = t0;
+    a.bounds[1] = t1;
+  }
+  if (e < a.E) a.woff[e + 1] = upto;
+  __syncthreads();
+  const int share = max(1, EW_THREADS / 32 / a.E);       // warps that share an expert's list
+  for (int x = warp / share; x < a.E; x += EW_THREADS / 32 / share)
+#pragma unroll 4
+    for (int i = start[x] + 32 * (warp % share) + lane; i < start[x + 1]; i += 32 * share) a.wtok[i] = a.tok[from[x] + i - start[x]];
 }
 
 struct DenseExpertsWs {
-  size_t tok, rw, pos, off, route, xs, z, wide, d, total;
-  DenseExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
-    const size_t A = static_cast<size_t>(T * k);
+  DenseRows scratch;
+  size_t tok, rw, pos, off, route, wtok, woff, bounds, xs, z, wide, d, total;
+  DenseExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) : scratch(T, k, E, H, I) {
+    const size_t A = static_cast<size_t>(T * k), R = static_cast<size_t>(scratch.rows);
     size_t at = 0;
     auto take = [&](size_t bytes) {
       const size_t here = at;
@@ -283,9 +374,12 @@ struct DenseExpertsWs {
     pos = take(A * 4);
     off = take(static_cast<size_t>(E + 1) * 4);
     route = take(bm_route_build_workspace_bytes(static_cast<int32_t>(T), static_cast<int32_t>(k), static_cast<int32_t>(E)));
-    z = take(A * I * 2);
-    wide = take(A * I * 4);
-    d = xs = take(A * H * 4);      // rows of x in expert order are read before the down products are written
+    wtok = take(scratch.step < T ? R * 4 : 0);
+    woff = take(static_cast<size_t>(E + 1) * 4);
+    bounds = take(8);
+    z = take(R * I * 2);
+    wide = take(R * I * 4);
+    d = xs = take(R * H * 4);      // rows of x in expert order are read before the down products are written
     total = at;
   }
 };
@@ -340,31 +434,47 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
              "dense_experts: workspace must be 256-byte aligned and hold %zu bytes (%zu given)", at.total, workspace_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  int32_t *tok = reinterpret_cast<int32_t*>(ws + at.tok), *off = reinterpret_cast<int32_t*>(ws + at.off);
-  const int A = T * k;
-  int rc = bm_route_build(topk_idx, topk_w, global_to_local, num_routed, T, k, num_local, 128, tok, off, reinterpret_cast<float*>(ws + at.rw), nullptr,
-                          nullptr, ws + at.route, at.z - at.route, stream);
+  int32_t *tok = reinterpret_cast<int32_t*>(ws + at.tok), *off = reinterpret_cast<int32_t*>(ws + at.off), *pos = reinterpret_cast<int32_t*>(ws + at.pos);
+  int32_t *wtok = reinterpret_cast<int32_t*>(ws + at.wtok), *woff = reinterpret_cast<int32_t*>(ws + at.woff), *bounds = reinterpret_cast<int32_t*>(ws + at.bounds);
+  const int A = T * k, rows = static_cast<int>(at.scratch.rows), step = at.scratch.step;
+  const bool windows = step < T, distinct = at.scratch.per < k;
+  SlotArgs slots{topk_idx, global_to_local, windows ? wtok : tok, windows ? woff : off, pos, A, k, num_local, num_routed, 0, distinct, windows ? bounds : nullptr};
+  if (distinct) {
+    BM_CUDA(launch_after(AFTER_READS, 1, experts_distinct_kernel, dim3((T + 7) / 8), 256, 0, st, slots, T, pos));       // until the places go there
+    BM_LAUNCH_CHECK("experts_distinct_kernel");
+  }
+  int rc = bm_route_build(distinct ? pos : topk_idx, topk_w, global_to_local, num_routed, T, k, num_local, 128, tok, off, reinterpret_cast<float*>(ws + at.rw), nullptr,
+                          nullptr, ws + at.route, at.wtok - at.route, stream);
   if (rc) return rc;
-  GroupedArgs g{};
-  g.x = x; g.w = w_gate_up; g.offsets = off; g.index = tok; g.y = ws + at.z;
-  g.x_rows = T; g.rows = A; g.K = hidden; g.N = intermediate; g.E = num_local; g.dtype = g.y_dtype = dtype; g.glu = 1;
-  g.expected = static_cast<int>(static_cast<int64_t>(A) * num_local / std::max(num_routed, num_local));
-  g.gathered = ws + at.xs;
-  g.wide = dtype == BM_F16 ? reinterpret_cast<float*>(ws + at.wide) : nullptr;
-  g.after = AFTER_READS;
-  if ((rc = launch_grouped(g, st))) return rc;
-  g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
-  g.x_rows = A; g.K = intermediate; g.N = hidden; g.glu = 0;
-  int32_t* pos = reinterpret_cast<int32_t*>(ws + at.pos);
-  g.slots = SlotArgs{topk_idx, global_to_local, tok, off, pos, A, k, num_local, num_routed, g.expected < A / 4};
-  if ((rc = launch_grouped(g, st))) return rc;
-  CombineArgs c{};
-  c.d = reinterpret_cast<const float*>(ws + at.d);
-  c.pos = pos; c.topk_w = topk_w; c.residual = residual; c.y = y; c.k = k; c.H = hidden;
-  c.slots = g.slots; c.z = ws + at.z; c.wide = reinterpret_cast<const float*>(ws + at.wide); c.w_down = w_down; c.I = intermediate;
-  c.vec = hidden % 4 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 7u) == 0;
-  BM_CUDA(launch_after(AFTER_READS, 1, dtype == BM_F16 ? experts_combine_kernel<BM_F16> : experts_combine_kernel<BM_BF16>,
-                       dim3(T, (hidden + 4 * EC_THREADS - 1) / (4 * EC_THREADS)), EC_THREADS, 0, st, c));
-  BM_LAUNCH_CHECK("experts_combine_kernel");
+  for (int64_t t = 0; t < T; t += windows ? step : T) {
+    if (windows) {
+      const WindowArgs w{tok, off, wtok, woff, bounds, T, num_local, rows, step, t == 0};
+      BM_CUDA(launch_after(AFTER_READS, 1, experts_window_kernel, dim3(1), EW_THREADS, 0, st, w));
+      BM_LAUNCH_CHECK("experts_window_kernel");
+    }
+    GroupedArgs g{};
+    g.x = x; g.w = w_gate_up; g.offsets = windows ? woff : off; g.index = windows ? wtok : tok; g.y = ws + at.z;
+    g.x_rows = T; g.rows = rows; g.K = hidden; g.N = intermediate; g.E = num_local; g.dtype = g.y_dtype = dtype; g.glu = 1;
+    g.expected = static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(A) * num_local / std::max(num_routed, num_local)));
+    g.gathered = ws + at.xs;
+    g.wide = dtype == BM_F16 ? reinterpret_cast<float*>(ws + at.wide) : nullptr;
+    g.after = AFTER_READS;
+    g.may_be_empty = t > 0;
+    if ((rc = launch_grouped(g, st))) return rc;
+    slots.sparse = g.expected < A / 4;
+    g.slots = slots;
+    g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
+    g.x_rows = rows; g.K = intermediate; g.N = hidden; g.glu = 0;
+    if ((rc = launch_grouped(g, st))) return rc;
+    CombineArgs c{};
+    c.d = reinterpret_cast<const float*>(ws + at.d);
+    c.pos = pos; c.topk_w = topk_w; c.residual = residual; c.y = y; c.T = T; c.k = k; c.H = hidden;
+    c.slots = g.slots; c.z = ws + at.z; c.wide = reinterpret_cast<const float*>(ws + at.wide); c.w_down = w_down; c.I = intermediate;
+    c.vec = hidden % 4 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 7u) == 0;
+    const int columns = (hidden + 4 * EC_THREADS - 1) / (4 * EC_THREADS);
+    BM_CUDA(launch_after(AFTER_READS, 1, dtype == BM_F16 ? experts_combine_kernel<BM_F16> : experts_combine_kernel<BM_BF16>,
+                         dim3(windows ? std::min(T, std::max(1, 1332 / columns)) : T, columns), EC_THREADS, 0, st, c));
+    BM_LAUNCH_CHECK("experts_combine_kernel");
+  }
   return BM_OK;
 }

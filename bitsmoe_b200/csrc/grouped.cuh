@@ -11,6 +11,8 @@ struct SlotArgs {
   int32_t* pos;                // [T * k]; null: nothing to do
   int slots, k, E, num_routed;
   int sparse;                  // most slots name experts that are not held here
+  int distinct;                // slots of a token that name one expert share a row
+  const int32_t* window;       // [2] tokens from, to: the others' slots are left alone; null: all
 };
 
 // y[i][n] = sum_k x[row(i)][k] * w[e][n][k] for offsets[e] <= i < offsets[e + 1], row(i) = index[i] (i itself when null).
@@ -29,6 +31,7 @@ struct GroupedArgs {
   int expected;                // rows that the groups are expected to have, 0 = `rows`
   void* gathered;              // with an index: room for [rows, K], 16-byte aligned, or null
   SlotArgs slots;              // worked out beside the products
+  int may_be_empty;            // offsets ascend, and offsets[E] = 0 is to be expected
   LaunchAfter after;
 };
 
@@ -49,8 +52,13 @@ __device__ __forceinline__ int slot_place(const SlotArgs& a, int i) {
     if (a.token_indices[mid] < t) lo = mid + 1;
     else hi = mid;
   }
-  for (int j = t * a.k; j < i; ++j) lo += slot_expert(a, j) == e;
+  if (!a.distinct)
+    for (int j = t * a.k; j < i; ++j) lo += slot_expert(a, j) == e;
   return lo;
+}
+
+__device__ __forceinline__ int2 slot_range(const SlotArgs& a) {
+  return a.window ? make_int2(__ldcg(a.window) * a.k, __ldcg(a.window + 1) * a.k) : make_int2(0, a.slots);
 }
 
 // The rows of group e, whatever the caller's table holds: inside [0, rows), ends not before they start.

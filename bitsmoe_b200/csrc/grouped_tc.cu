@@ -48,6 +48,7 @@ struct GcParams {
   DenseGuard guard;
   int x_rows, rows, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
   SlotArgs slots;
+  int may_be_empty;
 };
 
 // Copies into this CTA's shared memory, signalled on `bar` (shared::cluster address, of either CTA of the pair): four rows, tiles.
@@ -120,8 +121,10 @@ __device__ __forceinline__ GcItem gc_item(const GcTable& tab, int item, int& e) 
 // epilogue warps before their first item too.
 __device__ __forceinline__ void gc_places(const SlotArgs& a, int w, int lane) {
   const int warps = a.sparse ? 1 + GC_EPI_WARPS : 1;
-  if (a.pos && w < warps)
-    for (int i = (blockIdx.x * warps + w) * 32 + lane; i < a.slots; i += gridDim.x * warps * 32) a.pos[i] = slot_place(a, i);
+  if (a.pos && w < warps) {
+    const int2 r = slot_range(a);
+    for (int i = r.x + (blockIdx.x * warps + w) * 32 + lane; i < r.y; i += gridDim.x * warps * 32) a.pos[i] = slot_place(a, i);
+  }
 }
 
 template <bool BF16>
@@ -178,6 +181,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   tc::cluster_arrive();
   grid_launch_dependents();
   grid_wait();
+  if (p.may_be_empty && __ldg(p.offsets + p.E) == 0) {
+    tc::cluster_wait();
+    gc_places(p.slots, warp, lane);
+    return;
+  }
   for (int e = threadIdx.x; e < p.E; e += GC_THREADS) {
     const int2 r = group_rows(p.offsets, e, p.rows);
     t_start[e] = r.x;
@@ -506,6 +514,7 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
   p.slices = (a.K + GC_K - 1) / GC_K;
   p.vec = a.N % 8 == 0 && aligned16(a.y);
   p.slots = a.slots;
+  p.may_be_empty = a.may_be_empty;
   const bool f32 = a.y_dtype == BM_F32;
   if (f32 && (a.glu || a.index)) return BM_ERR_UNSUPPORTED;
   static PerDeviceOnce once;

@@ -271,7 +271,8 @@ BM_API int bm_grouped_linear(const void* x, int dtype, const void* w, int32_t x_
  * is not held here add nothing.  w_gate_up [num_local, 2 * intermediate, hidden], gate rows before up rows; w_down [num_local, hidden,
  * intermediate]; residual may be NULL.  k <= 32.  The sum runs in the order of the slots: two runs give the same bits.  The value between the
  * products is held in `dtype`; where that is fp16 and does not reach, the fp32 value is kept beside it and used.  The workspace holds
- * T * k rows of 4 * hidden + 6 * intermediate bytes and the routing lists, whatever share of the slots is held here. */
+ * T * k rows of 4 * hidden + 6 * intermediate bytes and the routing lists, whatever share of the slots is held here; T * min(k, num_local) rows where
+ * that would be more than 256 MB, and no more than 1 GB or four times the weights: longer batches go through in windows of tokens. */
 BM_API size_t bm_dense_experts_workspace_bytes(int32_t T, int32_t k, int32_t num_local, int32_t hidden, int32_t intermediate);
 BM_API int bm_dense_experts_forward(const void* x, int dtype, const int32_t* topk_idx, const float* topk_w, const int32_t* global_to_local,
                                     int32_t num_routed, int32_t T, int32_t k, int32_t num_local, const void* w_gate_up,
