@@ -455,7 +455,7 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
     GroupedArgs g{};
     g.x = x; g.w = w_gate_up; g.offsets = windows ? woff : off; g.index = windows ? wtok : tok; g.y = ws + at.z;
     g.x_rows = T; g.rows = rows; g.K = hidden; g.N = intermediate; g.E = num_local; g.dtype = g.y_dtype = dtype; g.glu = 1;
-    g.expected = static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(A) * num_local / std::max(num_routed, num_local)));
+    g.expected = static_cast<int>(std::min<int64_t>(rows, std::max<int64_t>(1, static_cast<int64_t>(A) * num_local / std::max(num_routed, num_local))));
     g.gathered = ws + at.xs;
     g.wide = dtype == BM_F16 ? reinterpret_cast<float*>(ws + at.wide) : nullptr;
     g.after = AFTER_READS;

@@ -208,6 +208,20 @@ def test_few_held_experts_of_many(dtype):
     assert torch.equal(got[none], res[none])
 
 
+@pytest.mark.parametrize("T", [24, 1, 300])
+def test_one_held_expert_of_many_takes_four_launches(T):
+    """Fewer rows expected than one: no pass over the rows of x before the products."""
+    x, idx, w, gu, dn = expert_case(13, T, 10, 1, 256, 64, torch.float16, routed=512)
+    g2l = torch.full((512,), -1, dtype=torch.int32, device=DEV)
+    g2l[idx[0, 0]] = 0
+    lib = capi.lib()
+    before = lib.bm_launch_count()
+    got = dense_experts(x, idx, w, gu, dn, global_to_local=g2l)
+    launches = lib.bm_launch_count() - before
+    db.check(got, *experts_exact(x, idx, w, gu, dn, g2l), what="one of 512")
+    assert launches == 4
+
+
 def test_chain_from_logits_as_a_block_runs_it():
     """Router tail, routing build, grouped products with the routed lists, and the whole as one call: the same numbers."""
     gen = torch.Generator().manual_seed(8)
