@@ -110,7 +110,10 @@ __global__ void __launch_bounds__(GR_THREADS) gather_rows_kernel(const uint4* __
                                                                  int E, int x_rows, int rows, int pieces, uint4* __restrict__ out) {
   grid_launch_dependents();
   grid_wait();
-  const int lane = threadIdx.x & 31, warps = gridDim.x * (GR_THREADS / 32), end = min(max(__ldg(offsets + E), 0), rows);
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (GR_THREADS / 32);
+  int end = 0;                 // behind the last row that a group owns: offsets[E], unless the table does not ascend
+  for (int e = lane; e < E; e += 32) end = max(end, group_rows(offsets, e, rows).y);
+  end = __reduce_max_sync(0xffffffffu, end);
   for (int64_t i0 = static_cast<int64_t>(blockIdx.x * (GR_THREADS / 32) + (threadIdx.x >> 5)) * GR_ROWS; i0 < end; i0 += static_cast<int64_t>(warps) * GR_ROWS) {
     const uint4* src[GR_ROWS];
 #pragma unroll

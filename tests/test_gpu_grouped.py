@@ -103,6 +103,18 @@ def test_indices_and_offsets_outside_their_ranges_are_harmless(K):
     db.check(out[3:], value[3:], err[3:], what="offsets outside")
 
 
+def test_offsets_that_descend_own_the_rows_before():
+    """[0, 500), then a group whose end lies before its start: long enough to be brought into order first, to scratch that holds NaN."""
+    gen = torch.Generator().manual_seed(14)
+    x, w = rnd(gen, 40, 64, dtype=torch.float16), rnd(gen, 2, 72, 64, std=0.1, dtype=torch.float16)
+    index = torch.randint(0, 40, (500,), generator=gen).to(torch.int32).to(DEV)
+    out = torch.zeros(500, 72, dtype=torch.float16, device=DEV)
+    poison = torch.full((500 * 64,), float("nan"), dtype=torch.float16, device=DEV)
+    del poison
+    grouped_linear(x, w, torch.tensor([0, 500, 400], dtype=torch.int32, device=DEV), index, out=out)
+    db.check(out, *grouped_exact(x, w, [500, 0], index), what="descending offsets")
+
+
 def test_nothing_to_do():
     x, w = torch.zeros(0, 64, dtype=torch.float16, device=DEV), torch.zeros(2, 32, 64, dtype=torch.float16, device=DEV)
     assert grouped_linear(x, w, offsets([0, 0])).shape == (0, 32)
