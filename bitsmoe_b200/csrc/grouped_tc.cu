@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
   }
   __syncthreads();
   tc::cluster_arrive();
-  grid_launch_dependents();
   grid_wait();
   if (p.may_be_empty && __ldg(p.offsets + p.E) == 0) {
     tc::cluster_wait();
@@ -192,7 +191,11 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     t_count[e] = r.y - r.x;
   }
   tc::cluster_wait();                          // both CTAs run and their barriers are set up
-  if (warp == 2) tc::tmem_alloc_pair(&tmem_slot, 512);
+  if (warp == 2) {
+    tc::tmem_alloc_pair(&tmem_slot, 512);
+    // not before: a launch that came to this SM ahead of the allocation could take tensor memory and then wait for this one
+    grid_launch_dependents();
+  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
