@@ -50,7 +50,8 @@ class _Symbol:
 
 
 class _StandIn:
-    """``self`` of the traced forward: the module with its Linears replaced by symbols; read-only."""
+    """``self`` of the traced forward: the module with its Linears replaced by symbols.  It hands out plain values, a configuration and
+    activations without state of their own, so that a forward that keeps a record of its calls neither runs nor passes."""
 
     def __init__(self, module):
         object.__setattr__(self, "_module", module)
@@ -58,7 +59,11 @@ class _StandIn:
     def __getattr__(self, name):
         if name in _NAMES:
             return lambda x: _Symbol(name, x) if isinstance(x, _Symbol) else NotImplemented
-        return getattr(self._module, name)
+        value = getattr(self._module, name)
+        if name == "config" or value is None or type(value) in (bool, int, float, str) or any(value is f for f in _SILU) or (
+                isinstance(value, nn.Module) and (type(value) is nn.SiLU or type(value).__module__ == "transformers.activations")):
+            return value
+        raise AttributeError(name)
 
     def __setattr__(self, name, value):
         raise AttributeError(name)

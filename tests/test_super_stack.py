@@ -198,6 +198,26 @@ class Noisy(DenseMLP):
         return self.down_proj(h + torch.randn_like(h) if self.noise else h)
 
 
+class Recording(DenseMLP):
+    def __init__(self, hidden, inter):
+        super().__init__(hidden, inter)
+        self.seen = []
+
+    def forward(self, x):
+        self.seen.append(x)
+        return DenseMLP.forward(self, x)
+
+
+class CountingSiLU(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.calls = 0
+
+    def forward(self, x):
+        self.calls += 1
+        return nn.functional.silu(x)
+
+
 class WithAct(DenseMLP):
     def __init__(self, hidden, inter, act):
         super().__init__(hidden, inter)
@@ -235,7 +255,8 @@ OTHER_KINDS = {
     "another activation in its forward": lambda: Gelu(HIDDEN, INTER).half(), "a clamp": lambda: Clamped(HIDDEN, INTER).half(),
     "gate and up the other way round": lambda: Swapped(HIDDEN, INTER).half(), "a factor": lambda: Scaled(HIDDEN, INTER).half(),
     "writes to itself": lambda: Counting(HIDDEN, INTER).half(), "an activation module": lambda: WithAct(HIDDEN, INTER, nn.GELU()).half(),
-    "an activation function": lambda: WithAct(HIDDEN, INTER, torch.tanh).half(), "a Linear of another class": low_rank, "a hook": hooked,
+    "an activation function": lambda: WithAct(HIDDEN, INTER, torch.tanh).half(), "a record of its calls": lambda: Recording(HIDDEN, INTER).half(),
+    "an activation that counts": lambda: WithAct(HIDDEN, INTER, CountingSiLU()).half(), "a Linear of another class": low_rank, "a hook": hooked,
     "a hook on a Linear": lambda: hooked("down_proj"), "a hook before it": lambda: hooked(pre=True), "a forward of its own": forward_of_its_own,
 }
 
@@ -246,6 +267,7 @@ def test_modules_of_another_kind_are_not_stacked(kind):
     blk = host_block({1: mlp(1), 4: other})
     where = [w.data_ptr() for w in weights(other)]
     assert blk._stacked_super_weights() is None and [w.data_ptr() for w in weights(other)] == where
+    assert not getattr(other, "seen", None) and not getattr(getattr(other, "act_fn", None), "calls", 0)
 
 
 def test_modules_that_are_swiglu_are_stacked():
