@@ -72,7 +72,13 @@ __global__ void __launch_bounds__(GG_THREADS) grouped_any_kernel(const GroupedAr
     for (int k0 = 0; k0 < a.K; k0 += GG_K) {
       for (int i = threadIdx.x; i < GG_ROWS * GG_K; i += GG_THREADS) {
         const int r = i / GG_K, k = i % GG_K;
-        xs[k][r] = src[r] >= 0 && k0 + k < a.K ? load16<D>(a.x, static_cast<int64_t>(src[r]) * a.K + k0 + k) : 0.f;
+        float v = 0.f;
+        if (src[r] >= 0 && k0 + k < a.K) {
+          const int64_t o = static_cast<int64_t>(src[r]) * a.K + k0 + k;
+          v = load16<D>(a.x, o);
+          if (!GLU && D == BM_F16 && a.x_wide && !(fabsf(v) <= 65504.f)) v = a.x_wide[o];
+        }
+        xs[k][r] = v;
       }
 #pragma unroll
       for (int h = 0; h < (GLU ? 2 : 1); ++h)
@@ -180,25 +186,8 @@ struct CombineArgs {
   const void* residual;
   void* y;
   int T, k, H, vec;            // vec: H % 4 == 0, y and the residual on 8-byte boundaries
-  // fp16: what the down product was made of
-  SlotArgs slots;
-  const void *z, *w_down;      // [rows, I], [E, H, I]
-  const float* wide;           // [rows, I], valid where z is not finite
-  int I;
+  const int32_t* window;       // [2] tokens from, to; null: all
 };
-// A column of a row of d from z's values before their rounding.  The product between the two matrices of an expert may pass fp16's range
-// where the sum over it does not: z is infinite there, and with it the row of d.
-__device__ __forceinline__ float wide_down(const CombineArgs& a, int slot, int64_t at, int h) {
-  const __half *z = static_cast<const __half*>(a.z) + at * a.I, *w = static_cast<const __half*>(a.w_down) + (static_cast<int64_t>(slot_expert(a.slots, slot)) * a.H + h) * a.I;
-  float v = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < a.I; ++i) {
-    float f = __half2float(z[i]);
-    if (!(fabsf(f) <= 65504.f)) f = a.wide[at * a.I + i];
-    v = fmaf(__half2float(w[i]), f, v);
-  }
-  return v;
-}
 template <int D>
 __device__ __forceinline__ float4 load4(const void* p, int64_t i) {
   const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
@@ -214,7 +203,7 @@ __global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const Combi
   grid_launch_dependents();
   grid_wait();
   if (h >= a.H) return;
-  const int2 tokens = a.slots.window ? make_int2(__ldcg(a.slots.window), __ldcg(a.slots.window + 1)) : make_int2(0, a.T);
+  const int2 tokens = a.window ? make_int2(__ldcg(a.window), __ldcg(a.window + 1)) : make_int2(0, a.T);
   for (int t = tokens.x + blockIdx.x; t < tokens.y; t += gridDim.x) {
     const int64_t o = static_cast<int64_t>(t) * a.H + h;
     const int n = min(4, a.H - h);
@@ -251,21 +240,6 @@ __global__ void __launch_bounds__(EC_THREADS) experts_combine_kernel(const Combi
         v[3] = fmaf(w[u], d[u].w, v[3]);
       }
     }
-    if (D == BM_F16 && !(fabsf((v[0] + v[1]) + (v[2] + v[3])) < __int_as_float(0x7f800000)))
-      // once more, slot by slot, with the rows of d that are not finite worked out anew
-#pragma unroll 1
-      for (int j = 0; j < n; ++j) {
-        float sum = a.residual ? load16<D>(a.residual, o + j) : 0.f;
-#pragma unroll 1
-        for (int s = 0; s < a.k; ++s) {
-          const int slot = t * a.k + s, at = a.pos[slot];
-          if (at < 0) continue;
-          float d = a.d[static_cast<int64_t>(at) * a.H + h + j];
-          if (!(fabsf(d) < __int_as_float(0x7f800000))) d = wide_down(a, slot, at, h + j);
-          sum = fmaf(a.topk_w[slot], d, sum);
-        }
-        v[0] = j == 0 ? sum : v[0]; v[1] = j == 1 ? sum : v[1]; v[2] = j == 2 ? sum : v[2]; v[3] = j == 3 ? sum : v[3];
-      }
     uint16_t out[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = D == BM_F16 ? __half_as_ushort(__float2half_rn(v[j])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
@@ -466,13 +440,15 @@ extern "C" int bm_dense_experts_forward(const void* x, int dtype, const int32_t*
     if ((rc = launch_grouped(g, st))) return rc;
     slots.sparse = g.expected < A / 4;
     g.slots = slots;
+    g.x_wide = g.wide;
+    g.wide = nullptr;
     g.x = g.y; g.w = w_down; g.index = nullptr; g.y = ws + at.d; g.y_dtype = BM_F32;
     g.x_rows = rows; g.K = intermediate; g.N = hidden; g.glu = 0;
     if ((rc = launch_grouped(g, st))) return rc;
     CombineArgs c{};
     c.d = reinterpret_cast<const float*>(ws + at.d);
     c.pos = pos; c.topk_w = topk_w; c.residual = residual; c.y = y; c.T = T; c.k = k; c.H = hidden;
-    c.slots = g.slots; c.z = ws + at.z; c.wide = reinterpret_cast<const float*>(ws + at.wide); c.w_down = w_down; c.I = intermediate;
+    c.window = slots.window;
     c.vec = hidden % 4 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 7u) == 0;
     const int columns = (hidden + 4 * EC_THREADS - 1) / (4 * EC_THREADS);
     BM_CUDA(launch_after(AFTER_READS, 1, dtype == BM_F16 ? experts_combine_kernel<BM_F16> : experts_combine_kernel<BM_BF16>,

@@ -28,6 +28,7 @@ struct GroupedArgs {
   int dtype, y_dtype;          // of x and w: BM_F16 or BM_BF16; of y: the same or BM_F32
   int glu;
   float* wide;                 // glu with fp16 y: [rows, N], gets the values that fp16 does not hold (their y is infinite); or null
+  const float* x_wide;         // such values of x (fp16, in order, fp32 y); or null
   int expected;                // rows that the groups are expected to have, 0 = `rows`
   void* gathered;              // with an index: room for [rows, K], 16-byte aligned, or null
   SlotArgs slots;              // worked out beside the products

@@ -45,8 +45,10 @@ struct GcParams {
   const int32_t* index;
   void* y;
   float* wide;
+  const float* x_wide;
+  const __half *xp, *wp;       // x and w, for the sums that x_wide makes necessary
   DenseGuard guard;
-  int x_rows, rows, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
+  int x_rows, rows, K, N, E, slices, vec, whole;     // vec: y takes 16-byte stores; whole: w describes a gated pair in blocks of 16 rows
   SlotArgs slots;
   int may_be_empty;
 };
@@ -141,12 +143,78 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// x is the product between the two matrices of an expert, which may pass fp16's range where the sums over it do not: x is infinite there, and with
+// it the whole row of y.  Such rows of this CTA's items are summed up here again, from x's values before their rounding, four columns a
+// warp; where those are infinite or not a number themselves y is what it should be.  Whole calls: one such token of 64 in 8 of 128 experts 204 -> 269 us, one
+// of 2048 in 6 of 64 322 -> 541, all 2048 of them 21 ms.
+__device__ __noinline__ void gc_redo(const GcParams& p, const GcTable& tab, int items, int width) {
+  __shared__ unsigned lost[GC_ROWS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, K = p.K;
+  const float inf = __int_as_float(0x7f800000);
+  float* const y = static_cast<float*>(p.y);
+  auto load8 = [](const __half* at, float (&v)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(at));
+    const __half2* e = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(e[j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  };
+  int e = 0;
+  for (int item = pair; item < items; item += pairs) {
+    const GcItem it = gc_item(tab, item, e);
+    const int col0 = (it.block * 2 + static_cast<int>(tc::cluster_rank())) * width, cols = min(width, p.N - col0);
+    __syncthreads();
+    if (threadIdx.x < GC_ROWS / 32) lost[threadIdx.x] = 0;
+    __syncthreads();
+    for (int r = warp; r < it.rows && cols > 0; r += GC_THREADS / 32) {
+      const int64_t row = it.row0 + r;
+      if (fabsf(__ldcg(y + row * p.N + col0)) < inf) continue;
+      bool mine = false;
+      for (int k = lane; k < K; k += 32)
+        if (!(fabsf(__half2float(p.xp[row * K + k])) <= 65504.f)) mine |= fabsf(p.x_wide[row * K + k]) < inf;
+      if (__any_sync(0xffffffffu, mine) && lane == 0) atomicOr(&lost[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    for (int r = 0; r < it.rows; ++r) {
+      if (!(lost[r >> 5] >> (r & 31) & 1u)) continue;
+      const int64_t row = it.row0 + r;
+      const __half *x = p.xp + row * K, *w = p.wp + (static_cast<int64_t>(it.e) * p.N + col0) * K;
+      for (int c0 = 4 * warp; c0 < cols; c0 += 4 * (GC_THREADS / 32)) {
+        float sum[4] = {};
+#pragma unroll 2
+        for (int k = 8 * lane; k < K; k += 256) {
+          float f[8], q[4][8];
+          load8(x + k, f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) load8(w + static_cast<int64_t>(min(c0 + c, cols - 1)) * K + k, q[c]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (!(fabsf(f[j]) <= 65504.f)) f[j] = p.x_wide[row * K + k + j];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = fmaf(q[c][j], f[j], sum[c]);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], o);
+          if (lane == c && c0 + c < cols) y[row * p.N + col0 + c0 + c] = sum[c];
+        }
+      }
+    }
+  }
+}
+
 // F32: y is fp32 (no gated pair).  GATHER: rows of x by index.
 template <bool GLU, bool GATHER, bool F32, bool BF16>
 __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_constant__ GcParams p) {
   extern __shared__ unsigned char gc_raw[];
   __shared__ __align__(8) uint64_t full[GC_MAX_STAGES], empty[GC_MAX_STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ int gave_up;                  // a wait of either CTA ran out
+  __shared__ int not_finite;               // a sum of this CTA is not
   __shared__ int issued[4];                // stages that either CTA's producers (2 rank, 2 rank + 1) have issued
   __shared__ uint32_t tmem_slot;
   __shared__ int longest;
@@ -163,6 +231,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
       tc::mbar_init(&empty[i], 1);
     }
     gave_up = p.guard.limit_ns == 0;
+    not_finite = 0;
     tc::mbar_init(&drained, 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
@@ -372,6 +441,12 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] += w[c];
           }
+          if (!BF16 && p.x_wide) {
+            float s = 0.f;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s += v[c];
+            if (!(fabsf(s) < __int_as_float(0x7f800000))) not_finite = 1;
+          }
           float* out = static_cast<float*>(p.y) + static_cast<int64_t>(it.row0 + c0) * p.N + col0 + lane;
           if (col0 + lane < p.N)
 #pragma unroll
@@ -476,6 +551,7 @@ __global__ void __launch_bounds__(GC_THREADS, 1) grouped_tc_kernel(const __grid_
     tc::cluster_wait();
   }
   if (warp == 2) tc::tmem_dealloc_pair(tmem_base, 512);
+  if (F32 && !BF16 && p.x_wide && not_finite) gc_redo(p, tab, items, quarters * 32);
 }
 
 static void (*const GC_KERNELS[])(const GcParams) = {
@@ -513,6 +589,7 @@ int launch_grouped_tc(const GroupedArgs& a, cudaStream_t st) {
     if (!encode_map16(&p.w, a.w, 3, dims, strides, box) || !encode_map16(&p.w32, a.w, 3, dims, strides, box32)) return BM_ERR_UNSUPPORTED;
   }
   p.offsets = a.offsets; p.index = a.index; p.y = a.y; p.wide = a.wide;
+  p.x_wide = a.x_wide; p.xp = static_cast<const __half*>(a.x); p.wp = static_cast<const __half*>(a.w); p.K = a.K;
   p.x_rows = a.x_rows; p.rows = a.rows; p.N = a.N; p.E = a.E;
   p.slices = (a.K + GC_K - 1) / GC_K;
   p.vec = a.N % 8 == 0 && aligned16(a.y);
