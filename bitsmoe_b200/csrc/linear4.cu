@@ -9,8 +9,8 @@
 // core and multiplied by the group's scale in fp32, so nothing but the output is rounded.  Few rows: the eight warps of a CTA and the
 // CTAs of a cluster share a row's columns and meet in shared memory, in a fixed order.
 //
-// Measured (groups of 128): K 2048, N 100003, 4 tokens 35.6 us in bf16 and 32 in fp16 (3.0 and 3.3 TB/s; floor 16.3): 40 instructions for 512 codes, with
-// four warps a scheduler.  K 2048, N 4096, one token 4.5 us inside a graph, 8192 x 8192 at 1 / 8 / 16 tokens 15 / 20 / 29 (floor 5.3).
+// Measured (groups of 128): K 2048, N 100003, 4 tokens 35.6 us in bf16 and 32 in fp16 (3.0 and 3.3 TB/s; floor 16.3): latency, since the
+// 40 instructions for 512 codes use 39 % of the issue slots: four warps a scheduler, each one chain of loads, unpacking, products and scale.  K 2048, N 4096, one token 4.5 us inside a graph, 8192 x 8192 at 1 / 8 / 16 tokens 15 / 20 / 29 (floor 5.3).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -403,7 +403,9 @@ static int linear4(Linear4Args a, int x_dtype, int group, LaunchAfter after, cud
   const bool fits = l4_smem_bytes(nt, a.K, a.splits, true) <= L4_SMEM_MOST && passes <= 65535;
   // More tokens than 16: passes over the weights side by side, or the tensor core's kernel, whichever has the smaller estimate (a wave of CTAs takes its
   // chunks and some four us).  us in passes / on the tensor core, bf16, groups of 128: K 512, N 2048, 64 tokens 6 / 11; 2048 x 2048, 32 tokens 9 / 13 and
-  // 48 tokens 14 / 14; K 2048, N 4096, 20 tokens 13 / 14 and 32 tokens 16 / 14; 4096 x 4096, 20 tokens 19 / 17; K 2048, N 16384, 20 tokens 25 / 19.
+  // 48 tokens 14 / 14; K 2048, N 4096, 20 tokens 13 / 14 and 32 tokens 16 / 14; 4096 x 4096, 20 tokens 19 / 17; K 2048, N 16384, 20 tokens 25 / 19.  Where
+  // the two are close the rule may take the slower (K 8192, N 2048, 20 tokens 21 / 24: estimates 25 / 23), and a gated pair's estimate is low (300 tokens,
+  // 2048 columns, 512 rows of each: 13, with a profiler 21).
   const double stream_us = ((a.row_blocks * a.splits * passes + sms * l4_ctas(nt) - 1) / (sms * l4_ctas(nt))) * (round + 4.0);
   if (!fits || (a.T > 16 && linear4_tc_us(a, sms) < stream_us)) {
     const int rc = launch_linear4_tc(a, x_dtype, group, after, st);

@@ -111,7 +111,7 @@ static __device__ __noinline__ void linear4_redo(const Linear4Args& a, int row0,
   }
 }
 // Finished sums of one row and up to C tokens: times the tokens' gates, plus the residual, out.  All loads are in flight before the
-// first store (one by one they cost 40 us of a product of 300 tokens, 512 x 2048).
+// first store (one by one a product of 300 tokens, 512 x 2048, with a residual took 22 us instead of 17).
 template <int XD, bool WIDE, int C, typename Token>      // WIDE: a.wide and a.x_wide are looked at
 __device__ __forceinline__ void linear4_finish(const Linear4Args& a, int row, const float (&v)[C], int& left_out, Token token) {      // token(i) < 0: none
   float f[C], r[C];

@@ -188,8 +188,10 @@ def patch_bitsmoe_inplace(model, bitsmoe_model_type: str, packed_state: Optional
 def quantize_dense_inplace(model, group_size: int = 128, projections: Sequence[str] = ("q_proj", "k_proj", "v_proj", "o_proj"),
                            shared_experts: bool = True) -> int:
     """Holds dense weights of a patched model in 4 bits: the bias-free Linears of its decoder layers that are named in ``projections``
-    (outside the MoE blocks), and the MoE blocks' shared experts.  Returns how many Linears were replaced.  The routed experts are packed
-    already, so these 16-bit matrices are most of what a decode step reads; routers, embeddings and the output layer stay as they are."""
+    (outside the MoE blocks), and the MoE blocks' shared experts.  Returns how many Linears were replaced.  Their weights take
+    about a quarter of the memory; few tokens also run faster, many slower: 2048 x 4096 in a graph takes 4.8 us for one token (torch's bf16
+    Linear 8.6), 6.3 for 8 (7.5), 15 for 64 (6.3) and 44 for 1024 (14); shared experts see ``quantize_shared_experts``.  Routers, embeddings and the
+    output layer stay as they are; ``Linear4.from_linear`` holds an output layer in 4 bits (100003 x 2048, one token: 35 us, bf16 98)."""
     n, inside = 0, set()
     for block in (m for m in model.modules() if isinstance(m, BitsMoE_BaseSparseMoeBlock)):
         inside.update(id(m) for m in block.modules())

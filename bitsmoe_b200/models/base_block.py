@@ -386,7 +386,8 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
 
     def quantize_shared_experts(self, group_size: int = 128) -> int:
         """Holds the shared expert's three Linears in 4 bits from now on (one scale for every ``group_size`` columns of a row); returns
-        how many were replaced.  At decode sizes their 16-bit weights are most of what such a layer reads."""
+        how many were replaced.  For memory, a quarter of theirs, not for speed: a Qwen3-Next block then leaves its one-call path and takes 43 us
+        instead of 33 for one token inside a graph, 88 instead of 72 for 64 (80 instead of 33 for one outside)."""
         n = 0
         for name in ("shared_expert", "shared_experts"):
             mlp = getattr(self, name, None)
