@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(EW_THREADS) experts_window_kernel(const Window
   __shared__ int from[EW_THREADS], sums[EW_THREADS / 32], start[EW_THREADS + 1];
   grid_launch_dependents();
   grid_wait();
-  const int e = threadIdx.x, lane = e & 31, warp = e >> 5, t0 = a.first ? 0 : a.bounds[1];
+  const int e = threadIdx.x, lane = e & 31, warp = e >> 5, t0 = a.first ? 0 : __ldcg(a.bounds + 1);
   const int begin = e < a.E ? a.off[e] : 0, end = e < a.E ? a.off[e + 1] : 0;
   auto first_of = [&](int t) {
     int lo = begin, hi = end;
