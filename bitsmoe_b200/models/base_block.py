@@ -25,7 +25,14 @@ from bitsmoe_b200.quant.linear4 import Linear4
 
 _FIELDS = ("payload", "rank_idx", "tile_meta", "slab_meta", "scale", "s")
 _TAGS = ("gate", "up", "down")
-_STACKING = threading.Lock()      # one for all blocks: an expert may belong to several, and a block is copied and pickled without it
+_STACKING: Dict[torch.device, threading.Lock] = {}
+
+
+def _stacking_lock(device: torch.device) -> threading.Lock:
+    """Of all blocks on a device: an expert may belong to several blocks, and a block is copied and pickled without it.  Not of all devices: who
+    holds it waits for its device, whose work may wait for a collective that the thread of another device has yet to launch."""
+    return _STACKING.setdefault(device, threading.Lock())
+
 
 
 class BitsMoE_BaseSparseMoeBlock(nn.Module):
@@ -239,7 +246,7 @@ class BitsMoE_BaseSparseMoeBlock(nn.Module):
             with torch.cuda.device(device):
                 if torch.cuda.is_current_stream_capturing():
                     return None                  # the copies would run at the graph's replay
-        with _STACKING:
+        with _stacking_lock(device):
             if not self._stack_holds(parts):     # else another thread has just built it
                 inter, hidden = parts[0][0].shape
                 with torch.inference_mode(False), torch.no_grad():    # the parameters stay ordinary tensors, whatever mode the first call is in

@@ -75,6 +75,33 @@ def test_threads_in_their_first_call_share_one_stack(monkeypatch):
     assert all(torch.equal(a, v) for a, v in zip((w for e in (1, 4, 6) for w in weights(blk.experts[e])), values))
 
 
+def test_devices_do_not_wait_for_one_another(monkeypatch):
+    """A thread that waits for its device while it stacks must not keep another device's thread from launching what it waits for."""
+    from bitsmoe_b200.models import base_block
+    blocks = {torch.device("cuda", 0): host_block({1: mlp(1)}), torch.device("cuda", 1): host_block({1: mlp(2)})}
+    both = threading.Barrier(2, timeout=20)
+    real, mine = getattr(base_block, "_stacking_lock", None), threading.local()
+    if real is not None:
+        monkeypatch.setattr(base_block, "_stacking_lock", lambda device: real(mine.device))
+    errors = []
+
+    def call(device):
+        mine.device = device
+        try:
+            blocks[device]._stacked_super_weights()
+        except threading.BrokenBarrierError as e:
+            errors.append(e)
+
+    for b in blocks.values():
+        monkeypatch.setattr(b, "_finish_copies", lambda device: both.wait())
+    threads = [threading.Thread(target=call, args=(d,)) for d in blocks]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+
+
 def test_loading_weights_keeps_the_stack():
     """What is loaded goes into the slices: the stack that a captured graph reads stays the one in use."""
     blk = host_block({1: mlp(1), 4: mlp(2)})
