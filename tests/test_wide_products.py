@@ -18,7 +18,7 @@ def largest(x, gate, up):
 
 
 @pytest.mark.parametrize("T,k,E,H,I", [(1, 8, 16, 256, 96), (7, 2, 5, 128, 40), (64, 4, 8, 256, 128), (333, 6, 12, 192, 72), (900, 8, 9, 128, 64),
-                                       (9, 2, 3, 65, 33), (40, 3, 4, 130, 47)])
+                                       (9, 2, 3, 65, 33), (40, 3, 4, 130, 47), (40, 3, 4, 130, 48), (40, 3, 4, 256, 47), (30001, 32, 32, 512, 64)])
 def test_dense_experts(T, k, E, H, I):
     x, idx, w, gu, dn = expert_case(16, T, k, E, H, I, FP16)
     rows = torch.arange(0, T, 3, device=DEV)
@@ -86,3 +86,23 @@ def test_dense_mlp4(tokens, hidden, inter, group, gated):
     others = torch.ones(tokens, dtype=torch.bool, device=DEV)
     others[rows] = False
     assert torch.equal(dense_mlp4(calm, packs[0], packs[1], down, group, token_gate_weight=tg, residual=res)[others], got[others])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 40, 300])
+def test_dense_mlp4_with_infinities(tokens):
+    """Rows of x, and scales of the down matrix, that are infinite or not a number keep to their rows and columns."""
+    x, packs, mats, tg, res = mlp_case(9, tokens, 512, 352, 64, FP16)
+    want = dense_mlp4(x, *packs, 64, token_gate_weight=tg, residual=res)
+    bad = x.clone()
+    bad[0, 3] = float("nan")
+    bad[tokens // 2, 5] = float("inf")
+    rows = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    rows[[0, tokens // 2]] = False
+    got = dense_mlp4(bad, *packs, 64, token_gate_weight=tg, residual=res)
+    assert torch.equal(got[rows], want[rows]) and not bool(got[~rows].isfinite().any())
+    scale = packs[2][1].clone()
+    scale[7, 2], scale[300, 0] = float("inf"), float("nan")
+    cols = torch.ones(512, dtype=torch.bool, device=DEV)
+    cols[[7, 300]] = False
+    got = dense_mlp4(x, packs[0], packs[1], (packs[2][0], scale), 64, token_gate_weight=tg, residual=res)
+    assert torch.equal(got[:, cols], want[:, cols]) and not bool(got[:, ~cols].isfinite().any())
